@@ -65,6 +65,16 @@ lib.bgemm_gemm_auto_split_k.argtypes = [_i64, _i64, _i64, _i64]
 lib.bgemm_linear_forward.argtypes = [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _int, _vp, _int, _vp, _sz]
 lib.bgemm_linear_workspace_bytes.restype = _sz
 lib.bgemm_linear_workspace_bytes.argtypes = [_i64, _i64, _i64, _int]
+lib.bgemm_w4_row_bytes.restype = _i64
+lib.bgemm_w4_row_bytes.argtypes = [_i64]
+lib.bgemm_w4_quantize.argtypes = [_vp, _vp, _int, _i64, _i64, _i64, _int, _int, _int, _vp, _vp, _vp, _i64, _i64]
+lib.bgemm_w4_dequantize.argtypes = [_vp, _vp, _i64, _i64, _int, _vp, _vp, _int, _vp]
+lib.bgemm_w4a16_gemm.argtypes = [_vp, _vp, _i64, _i64, _int, _vp, _vp, _vp, _i64, _int, _i64, _vp, _i64]
+lib.bgemm_w4a16_grouped_gemm.argtypes = [_vp, _vp, _i64, _i64, _i64, _int, _vp, _vp, _vp, _i64, _i64, _int, _vp, _vp, _i64, _vp, _i64]
+lib.bgemm_moe_route_workspace_bytes.restype = _sz
+lib.bgemm_moe_route_workspace_bytes.argtypes = [_i64, _i64]
+lib.bgemm_moe_route.argtypes = [_vp, _vp, _int, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp, _vp, _vp, _vp, _sz]
+lib.bgemm_moe_combine.argtypes = [_vp, _vp, _int, _i64, _i64, _i64, _vp, _vp, _i64, _int, _vp, _i64]
 lib.bgemm_device_status.restype = _int
 lib.bgemm_device_status.argtypes = [_int]
 lib.bgemm_debug_set_wait_test.restype = None

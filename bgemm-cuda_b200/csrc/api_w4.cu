@@ -1,0 +1,129 @@
+// extern "C" surface of the 4-bit weight products and the expert routing (include/bgemm_b200.h): argument checks and launches.
+#include "internal.h"
+#include "w4.cuh"
+
+using namespace bgemm;
+
+namespace {
+constexpr long long kMaxDim = 1LL << 24;
+constexpr long long kMaxSlots = 1LL << 30;       // rows of a grouped product, pairs of a routing call
+constexpr int kMaxExperts = 1024, kMaxTopK = 32;
+
+bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+bool group_ok(int g) { return g == 32 || g == 64 || g == 128; }
+bool is16(int d) { return d == BGEMM_DT_F16 || d == BGEMM_DT_BF16; }
+
+int check_matrix(int64_t M, int64_t K, int group) {
+    if (!group_ok(group)) return BGEMM_ERR_ENUM;
+    if (M < 1 || K < 1 || M > kMaxDim || K > kMaxDim) return BGEMM_ERR_SHAPE;
+    return BGEMM_OK;
+}
+
+int check_gemm(const void* plane, int64_t M, int64_t K, int group, const void* scales, const void* x, int64_t x_ld, int64_t x_rows, int dtype,
+               int64_t slots, const void* out, int64_t out_ld) {
+    if (!plane || !scales || !x || !out) return BGEMM_ERR_NULL;
+    if (!is16(dtype)) return BGEMM_ERR_ENUM;
+    const int rc = check_matrix(M, K, group);
+    if (rc) return rc;
+    if (slots < 1 || slots > kMaxSlots || x_rows < 1 || x_rows > kMaxSlots || x_ld < K || out_ld < M || x_ld > (1LL << 40) || out_ld > (1LL << 40))
+        return BGEMM_ERR_SHAPE;
+    if (!aligned(plane, 16) || !aligned(scales, 2) || !aligned(x, 2) || !aligned(out, 2)) return BGEMM_ERR_ALIGN;
+    return BGEMM_OK;
+}
+
+W4Gemm problem(const void* plane, int E, int64_t M, int64_t K, int group, const void* scales, const void* zeros, const void* x, int64_t x_ld,
+               int64_t x_rows, int64_t slots, void* out, int64_t out_ld) {
+    W4Gemm p{};
+    p.plane = static_cast<const uint8_t*>(plane);
+    p.scales = static_cast<const uint16_t*>(scales);
+    p.zeros = static_cast<const uint8_t*>(zeros);
+    p.x = x;
+    p.out = out;
+    p.row_bytes = bgemm_w4_row_bytes(K);
+    p.x_ld = x_ld; p.x_rows = x_rows; p.out_ld = out_ld; p.slots = slots;
+    p.E = E; p.M = (int)M; p.K = (int)K; p.group = group; p.groups = (int)((K + group - 1) / group);
+    p.x_vec = aligned(x, 16) && (x_rows == 1 || x_ld % 8 == 0);
+    return p;
+}
+}  // namespace
+
+extern "C" {
+
+int64_t bgemm_w4_row_bytes(int64_t K) { return K < 1 ? 0 : (K + kW4Block - 1) / kW4Block * kW4BlockBytes; }
+
+int bgemm_w4_quantize(void* stream, const void* src, int src_dtype, int64_t M, int64_t K, int64_t ld, int group, int symmetric, int scale_dtype,
+                      void* plane, void* scales, uint8_t* zeros, int64_t batch, int64_t src_batch_stride) {
+    if (!src || !plane || !scales || (!symmetric && !zeros)) return BGEMM_ERR_NULL;
+    if (src_dtype < BGEMM_DT_F16 || src_dtype > BGEMM_DT_F32 || !is16(scale_dtype)) return BGEMM_ERR_ENUM;
+    const int rc = check_matrix(M, K, group);
+    if (rc) return rc;
+    if (ld < K || ld > (1LL << 40) || batch < 1 || batch > 65535 || (batch > 1 && src_batch_stride < 0)) return BGEMM_ERR_SHAPE;
+    if (!aligned(plane, 16) || !aligned(scales, 2) || !aligned(src, src_dtype == BGEMM_DT_F32 ? 4 : 2)) return BGEMM_ERR_ALIGN;
+    return launch_w4_quantize((cudaStream_t)stream, src, src_dtype, M, K, ld, group, symmetric ? 1 : 0, scale_dtype, plane, scales,
+                              symmetric ? nullptr : zeros, batch, src_batch_stride);
+}
+
+int bgemm_w4_dequantize(void* stream, const void* plane, int64_t M, int64_t K, int group, const void* scales, const uint8_t* zeros, int dtype,
+                        void* out) {
+    if (!plane || !scales || !out) return BGEMM_ERR_NULL;
+    if (!is16(dtype)) return BGEMM_ERR_ENUM;
+    if (!group_ok(group)) return BGEMM_ERR_ENUM;
+    if (M < 1 || K < 1 || M > (1LL << 40) || K > kMaxDim) return BGEMM_ERR_SHAPE;      // M: all rows of a stack of matrices
+    if (!aligned(plane, 16) || !aligned(scales, 2) || !aligned(out, 2)) return BGEMM_ERR_ALIGN;
+    return launch_w4_dequantize((cudaStream_t)stream, plane, M, K, group, scales, zeros, dtype, out);
+}
+
+int bgemm_w4a16_gemm(void* stream, const void* plane, int64_t M, int64_t K, int group, const void* scales, const uint8_t* zeros, const void* x,
+                     int64_t x_ld, int dtype, int64_t N, void* out, int64_t out_ld) {
+    const int rc = check_gemm(plane, M, K, group, scales, x, x_ld, N, dtype, N, out, out_ld);
+    if (rc) return rc;
+    const W4Gemm p = problem(plane, 1, M, K, group, scales, zeros, x, x_ld, N, N, out, out_ld);
+    return launch_w4_stream((cudaStream_t)stream, p, dtype);
+}
+
+int bgemm_w4a16_grouped_gemm(void* stream, const void* plane, int64_t E, int64_t M, int64_t K, int group, const void* scales, const uint8_t* zeros,
+                             const void* x, int64_t x_rows, int64_t x_ld, int dtype, const int32_t* offsets, const int32_t* rows, int64_t slots,
+                             void* out, int64_t out_ld) {
+    if (!offsets) return BGEMM_ERR_NULL;
+    const int rc = check_gemm(plane, M, K, group, scales, x, x_ld, x_rows, dtype, slots, out, out_ld);
+    if (rc) return rc;
+    if (E < 1 || E > kMaxExperts || (!rows && x_rows < slots)) return BGEMM_ERR_SHAPE;
+    if (!aligned(offsets, 4) || !aligned(rows, 4)) return BGEMM_ERR_ALIGN;
+    W4Gemm p = problem(plane, (int)E, M, K, group, scales, zeros, x, x_ld, x_rows, slots, out, out_ld);
+    p.offsets = offsets;
+    p.rows = rows;
+    return launch_w4_stream((cudaStream_t)stream, p, dtype);
+}
+
+size_t bgemm_moe_route_workspace_bytes(int64_t T, int64_t E) {
+    if (T < 1 || E < 1 || E > kMaxExperts || T > kMaxSlots) return 0;
+    return moe_route_workspace(T, (int)E);
+}
+
+int bgemm_moe_route(void* stream, const void* logits, int dtype, int64_t T, int64_t E, int64_t ld, int top_k, int renormalize, float* weights,
+                    int32_t* experts, int32_t* offsets, int32_t* rows, int32_t* slots, void* workspace, size_t workspace_bytes) {
+    if (!logits || !weights || !experts || !offsets || !rows || !slots) return BGEMM_ERR_NULL;
+    if (dtype < BGEMM_DT_F16 || dtype > BGEMM_DT_F32) return BGEMM_ERR_ENUM;
+    if (T < 1 || E < 1 || E > kMaxExperts || ld < E || ld > (1LL << 40) || top_k < 1 || top_k > kMaxTopK || top_k > E || T > kMaxSlots / top_k)
+        return BGEMM_ERR_SHAPE;
+    if (!aligned(logits, dtype == BGEMM_DT_F32 ? 4 : 2) || !aligned(weights, 4) || !aligned(experts, 4) || !aligned(offsets, 4) || !aligned(rows, 4) ||
+        !aligned(slots, 4) || !aligned(workspace, 4))
+        return BGEMM_ERR_ALIGN;
+    const size_t need = moe_route_workspace(T, (int)E);
+    if (need && (!workspace || workspace_bytes < need)) return BGEMM_ERR_WORKSPACE;
+    return launch_moe_route((cudaStream_t)stream, logits, dtype, T, (int)E, ld, top_k, renormalize ? 1 : 0, weights, experts, offsets, rows, slots,
+                            static_cast<int32_t*>(workspace));
+}
+
+int bgemm_moe_combine(void* stream, const void* y, int dtype, int64_t slots_total, int64_t M, int64_t y_ld, const int32_t* slots, const float* weights,
+                      int64_t T, int top_k, void* out, int64_t out_ld) {
+    if (!y || !slots || !weights || !out) return BGEMM_ERR_NULL;
+    if (!is16(dtype)) return BGEMM_ERR_ENUM;
+    if (slots_total < 1 || slots_total > kMaxSlots || M < 1 || M > kMaxDim || y_ld < M || out_ld < M || y_ld > (1LL << 40) || out_ld > (1LL << 40) ||
+        top_k < 1 || top_k > kMaxTopK || T < 1 || T > kMaxSlots / top_k)
+        return BGEMM_ERR_SHAPE;
+    if (!aligned(y, 2) || !aligned(out, 2) || !aligned(slots, 4) || !aligned(weights, 4)) return BGEMM_ERR_ALIGN;
+    return launch_moe_combine((cudaStream_t)stream, y, dtype, slots_total, M, y_ld, slots, weights, T, top_k, out, out_ld);
+}
+
+}  // extern "C"

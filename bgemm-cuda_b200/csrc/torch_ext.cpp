@@ -325,6 +325,183 @@ torch::Tensor w1a16_linear_forward(torch::Tensor x, torch::Tensor plane, int64_t
     return out;
 }
 
+// ---- 4-bit weights and expert routing --------------------------------------------------------------------------
+int code16(const torch::Tensor& t, const char* where) {
+    TORCH_CHECK(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, where, ": float16 or bfloat16 required, got ", t.scalar_type());
+    return t.scalar_type() == at::kHalf ? BGEMM_DT_F16 : BGEMM_DT_BF16;
+}
+
+void check_group(int64_t group, const char* where) { TORCH_CHECK(group == 32 || group == 64 || group == 128, where, ": group_size must be 32, 64 or 128"); }
+
+// plane [.., M, row bytes], scales [.., M, groups], zeros the same as scales; all contiguous, on x's device
+void check_w4(const torch::Tensor& plane, const torch::Tensor& scales, const c10::optional<torch::Tensor>& zeros, int64_t K, int64_t group,
+              const torch::Device& dev, const char* where) {
+    check_group(group, where);
+    TORCH_CHECK(plane.is_cuda() && plane.device() == dev && scales.device() == dev, where, ": all tensors must be on one CUDA device");
+    TORCH_CHECK(plane.scalar_type() == at::kByte && plane.is_contiguous() && scales.is_contiguous(), where,
+                ": the plane must be uint8; plane and scales must be contiguous");
+    TORCH_CHECK(plane.dim() == scales.dim() && plane.dim() >= 2 && K >= 1 && plane.size(-1) == bgemm_w4_row_bytes(K) && scales.size(-1) == (K + group - 1) / group,
+                where, ": plane must be [.., M, w4_row_bytes(K)] and scales [.., M, ceil(K / group_size)]");
+    for (int64_t d = 0; d + 1 < plane.dim(); d++) TORCH_CHECK(plane.size(d) == scales.size(d), where, ": plane and scales have different shapes");
+    code16(scales, where);
+    if (zeros.has_value())
+        TORCH_CHECK(zeros->device() == dev && zeros->scalar_type() == at::kByte && zeros->is_contiguous() && zeros->sizes() == scales.sizes(), where,
+                    ": zeros must be contiguous uint8 of the scales' shape");
+}
+
+uint8_t* zeros_ptr(const c10::optional<torch::Tensor>& zeros) { return zeros.has_value() ? zeros->data_ptr<uint8_t>() : nullptr; }
+
+void no_grad_only(const torch::Tensor& t, const char* where) {
+    TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), where, ": forward only (no gradient): call it under torch.no_grad() or detach its input");
+}
+
+// [M, K] or [E, M, K] weights -> (plane uint8 [.., M, w4_row_bytes(K)], scales [.., M, groups], zeros uint8 [.., M, groups] or None).
+// The scales take the weights' type, fp16 for fp32 weights unless scale_bf16.
+py::tuple w4_quantize(torch::Tensor w, int64_t group, bool symmetric, bool scale_bf16) {
+    const char* where = "w4_quantize";
+    TORCH_CHECK(w.is_cuda() && (w.dim() == 2 || w.dim() == 3), where, ": 2-D or 3-D CUDA tensor required");
+    TORCH_CHECK(w.scalar_type() == at::kHalf || w.scalar_type() == at::kBFloat16 || w.scalar_type() == at::kFloat, where,
+                ": float16, bfloat16 or float32 weights required, got ", w.scalar_type());
+    check_group(group, where);
+    TORCH_CHECK(w.numel() > 0, where, ": empty matrix");
+    no_grad_only(w, where);
+    c10::cuda::CUDAGuard guard(w.device());
+    if (w.stride(-1) != 1 || (w.size(-2) > 1 && w.stride(-2) < w.size(-1))) w = w.contiguous();
+    const bool batched = w.dim() == 3;
+    const int64_t B = batched ? w.size(0) : 1, M = w.size(-2), K = w.size(-1), G = (K + group - 1) / group;
+    const auto kind = w.scalar_type() == at::kFloat ? (scale_bf16 ? at::kBFloat16 : at::kHalf) : w.scalar_type();
+    auto shaped = [&](int64_t last) { return batched ? std::vector<int64_t>{B, M, last} : std::vector<int64_t>{M, last}; };
+    const auto bytes = torch::TensorOptions().dtype(torch::kUInt8).device(w.device());
+    auto plane = torch::empty(shaped(bgemm_w4_row_bytes(K)), bytes);
+    auto scales = torch::empty(shaped(G), bytes.dtype(kind));
+    torch::Tensor zeros;
+    if (!symmetric) zeros = torch::empty(shaped(G), bytes);
+    check(bgemm_w4_quantize(stream_of(w), w.data_ptr(), dtype_code(w), M, K, M > 1 ? w.stride(-2) : K, (int)group, symmetric ? 1 : 0, dtype_code(scales),
+                            plane.data_ptr(), scales.data_ptr(), symmetric ? nullptr : zeros.data_ptr<uint8_t>(), B, batched && B > 1 ? w.stride(0) : 0),
+          "bgemm_w4_quantize");
+    return symmetric ? py::make_tuple(plane, scales, py::none()) : py::make_tuple(plane, scales, zeros);
+}
+
+torch::Tensor w4_dequantize(torch::Tensor plane, torch::Tensor scales, c10::optional<torch::Tensor> zeros, int64_t K, int64_t group) {
+    check_w4(plane, scales, zeros, K, group, plane.device(), "w4_dequantize");
+    c10::cuda::CUDAGuard guard(plane.device());
+    auto shape = plane.sizes().vec();
+    shape.back() = K;
+    auto out = torch::empty(shape, scales.options());
+    if (out.numel() == 0) return out;
+    check(bgemm_w4_dequantize(stream_of(plane), plane.data_ptr(), out.numel() / K, K, (int)group, scales.data_ptr(), zeros_ptr(zeros), dtype_code(scales),
+                              out.data_ptr()),
+          "bgemm_w4_dequantize");
+    return out;
+}
+
+// x [N, K] times a 4-bit matrix -> [N, M] of x's type (which is the scales' type too).
+torch::Tensor w4a16_linear_forward(torch::Tensor x, torch::Tensor plane, torch::Tensor scales, c10::optional<torch::Tensor> zeros, int64_t group) {
+    const char* where = "w4a16_linear_forward";
+    TORCH_CHECK(x.is_cuda() && x.dim() == 2 && plane.dim() == 2, where, ": x must be a CUDA tensor [N, K] and the plane [M, bytes]");
+    TORCH_CHECK(x.scalar_type() == scales.scalar_type(), where, ": x and the scales must have one type");
+    const int64_t N = x.size(0), K = x.size(1), M = plane.size(0);
+    check_w4(plane, scales, zeros, K, group, x.device(), where);
+    no_grad_only(x, where);
+    c10::cuda::CUDAGuard guard(x.device());
+    if (x.stride(1) != 1 || (N > 1 && x.stride(0) < K)) x = x.contiguous();
+    auto out = torch::empty({N, M}, x.options());
+    if (out.numel() == 0) return out;
+    check(bgemm_w4a16_gemm(stream_of(x), plane.data_ptr(), M, K, (int)group, scales.data_ptr(), zeros_ptr(zeros), x.data_ptr(), N > 1 ? x.stride(0) : K,
+                           dtype_code(x), N, out.data_ptr(), M),
+          "bgemm_w4a16_gemm");
+    return out;
+}
+
+// The same product by expert: plane [E, M, bytes], offsets int32 [E + 1], rows int32 [slots] or None (slot s reads row s of x).
+// Rows of the result behind offsets[E] are not written; `out` gives a buffer [slots, M] to write into.
+torch::Tensor w4a16_grouped_forward(torch::Tensor x, torch::Tensor plane, torch::Tensor scales, c10::optional<torch::Tensor> zeros, torch::Tensor offsets,
+                                    c10::optional<torch::Tensor> rows, int64_t group, c10::optional<torch::Tensor> out_opt) {
+    const char* where = "w4a16_grouped_forward";
+    TORCH_CHECK(x.is_cuda() && x.dim() == 2 && plane.dim() == 3, where, ": x must be a CUDA tensor [rows, K] and the plane [E, M, bytes]");
+    TORCH_CHECK(x.scalar_type() == scales.scalar_type(), where, ": x and the scales must have one type");
+    const int64_t K = x.size(1), E = plane.size(0), M = plane.size(1);
+    check_w4(plane, scales, zeros, K, group, x.device(), where);
+    no_grad_only(x, where);
+    TORCH_CHECK(offsets.device() == x.device() && offsets.scalar_type() == at::kInt && offsets.is_contiguous() && offsets.dim() == 1 && offsets.size(0) == E + 1,
+                where, ": offsets must be a contiguous int32 tensor [E + 1] on x's device");
+    if (rows.has_value())
+        TORCH_CHECK(rows->device() == x.device() && rows->scalar_type() == at::kInt && rows->is_contiguous() && rows->dim() == 1, where,
+                    ": rows must be a contiguous int32 tensor on x's device");
+    const int64_t slots = rows.has_value() ? rows->size(0) : x.size(0);
+    c10::cuda::CUDAGuard guard(x.device());
+    if (x.stride(1) != 1 || (x.size(0) > 1 && x.stride(0) < K)) x = x.contiguous();
+    torch::Tensor out;
+    if (out_opt.has_value()) {
+        out = *out_opt;
+        TORCH_CHECK(out.device() == x.device() && out.scalar_type() == x.scalar_type() && out.dim() == 2 && out.size(0) == slots && out.size(1) == M &&
+                        out.stride(1) == 1 && (slots <= 1 || out.stride(0) >= M),
+                    where, ": out must be a row-major [slots, M] tensor of x's type and device");
+    } else {
+        out = torch::empty({slots, M}, x.options());
+    }
+    if (out.numel() == 0 || x.size(0) == 0) {
+        TORCH_CHECK(out.numel() == 0, where, ": x has no rows");
+        return out;
+    }
+    check(bgemm_w4a16_grouped_gemm(stream_of(x), plane.data_ptr(), E, M, K, (int)group, scales.data_ptr(), zeros_ptr(zeros), x.data_ptr(), x.size(0),
+                                   x.size(0) > 1 ? x.stride(0) : K, dtype_code(x), offsets.data_ptr<int>(),
+                                   rows.has_value() ? rows->data_ptr<int>() : nullptr, slots, out.data_ptr(), slots > 1 ? out.stride(0) : M),
+          "bgemm_w4a16_grouped_gemm");
+    return out;
+}
+
+// logits [T, E] -> (weights fp32 [T, k], experts int32 [T, k], offsets int32 [E + 1], rows int32 [T k], slots int32 [T, k]); see bgemm_moe_route.
+std::vector<torch::Tensor> moe_route(torch::Tensor logits, int64_t top_k, bool renormalize) {
+    const char* where = "moe_route";
+    TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, where, ": a 2-D CUDA tensor [T, E] is required");
+    TORCH_CHECK(logits.scalar_type() == at::kHalf || logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kFloat, where,
+                ": float16, bfloat16 or float32 logits required, got ", logits.scalar_type());
+    const int64_t T = logits.size(0), E = logits.size(1);
+    TORCH_CHECK(E >= 1 && E <= 1024 && top_k >= 1 && top_k <= 32 && top_k <= E, where, ": 1 <= top_k <= min(E, 32) and E <= 1024 required");
+    no_grad_only(logits, where);
+    c10::cuda::CUDAGuard guard(logits.device());
+    if (logits.stride(1) != 1 || (T > 1 && logits.stride(0) < E)) logits = logits.contiguous();
+    const auto ints = torch::TensorOptions().dtype(at::kInt).device(logits.device());
+    auto weights = torch::empty({T, top_k}, ints.dtype(at::kFloat));
+    auto experts = torch::empty({T, top_k}, ints);
+    if (T == 0) return {weights, experts, torch::zeros({E + 1}, ints), torch::empty({0}, ints), torch::empty({T, top_k}, ints)};
+    auto offsets = torch::empty({E + 1}, ints);
+    auto rows = torch::empty({T * top_k}, ints);
+    auto slots = torch::empty({T, top_k}, ints);
+    const size_t need = bgemm_moe_route_workspace_bytes(T, E);
+    torch::Tensor ws;
+    if (need) ws = torch::empty({(int64_t)need}, ints.dtype(torch::kUInt8));
+    check(bgemm_moe_route(stream_of(logits), logits.data_ptr(), dtype_code(logits), T, E, T > 1 ? logits.stride(0) : E, (int)top_k, renormalize ? 1 : 0,
+                          weights.data_ptr<float>(), experts.data_ptr<int>(), offsets.data_ptr<int>(), rows.data_ptr<int>(), slots.data_ptr<int>(),
+                          need ? ws.data_ptr() : nullptr, need),
+          "bgemm_moe_route");
+    return {weights, experts, offsets, rows, slots};
+}
+
+// out[t] = sum_j weights[t, j] * y[slots[t, j]]
+torch::Tensor moe_combine(torch::Tensor y, torch::Tensor slots, torch::Tensor weights) {
+    const char* where = "moe_combine";
+    TORCH_CHECK(y.is_cuda() && y.dim() == 2 && slots.dim() == 2, where, ": y must be a CUDA tensor [slots, M] and slots [T, k]");
+    code16(y, where);
+    TORCH_CHECK(slots.device() == y.device() && weights.device() == y.device() && slots.scalar_type() == at::kInt && weights.scalar_type() == at::kFloat &&
+                    slots.is_contiguous() && weights.is_contiguous() && slots.sizes() == weights.sizes(),
+                where, ": slots (int32) and weights (float32) must be contiguous tensors [T, k] on y's device");
+    TORCH_CHECK(slots.size(1) >= 1 && slots.size(1) <= 32, where, ": 1 to 32 slots per token");
+    no_grad_only(y, where);
+    no_grad_only(weights, where);
+    c10::cuda::CUDAGuard guard(y.device());
+    const int64_t T = slots.size(0), M = y.size(1);
+    if (y.size(0) == 0) return torch::zeros({T, M}, y.options());
+    if (y.stride(1) != 1 || (y.size(0) > 1 && y.stride(0) < M)) y = y.contiguous();
+    auto out = torch::empty({T, M}, y.options());
+    if (out.numel() == 0) return out;
+    check(bgemm_moe_combine(stream_of(y), y.data_ptr(), dtype_code(y), y.size(0), M, y.size(0) > 1 ? y.stride(0) : M, slots.data_ptr<int>(),
+                            weights.data_ptr<float>(), T, (int)slots.size(1), out.data_ptr(), M),
+          "bgemm_moe_combine");
+    return out;
+}
+
 torch::Tensor fp6_not_provided(py::args, py::kwargs) {
     throw py::type_error("the FP6 entry points of the reference (linear_forward_cuda, weight_dequant_cpu) are not part of this library");
 }
@@ -360,6 +537,19 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("exact") = false);
     m.def("w1a16_linear_forward", &w1a16_linear_forward, "Binary weight x fp16 activation, fp32 accumulation.", py::arg("x"), py::arg("plane"),
           py::arg("M"), py::arg("K"), py::arg("alpha") = py::none(), py::arg("out_f32") = false, py::arg("static_weights") = false);
+    m.def("w4_quantize", &w4_quantize, "Weights -> (4-bit plane, scales, zeros or None).", py::arg("w"), py::arg("group_size") = 128,
+          py::arg("symmetric") = false, py::arg("scale_bf16") = false);
+    m.def("w4_dequantize", &w4_dequantize, "Values of a 4-bit plane in the scales' type.", py::arg("plane"), py::arg("scales"), py::arg("zeros"),
+          py::arg("K"), py::arg("group_size") = 128);
+    m.def("w4a16_linear_forward", &w4a16_linear_forward, "16-bit activations x 4-bit weights, fp32 accumulation.", py::arg("x"), py::arg("plane"),
+          py::arg("scales"), py::arg("zeros") = py::none(), py::arg("group_size") = 128);
+    m.def("w4a16_grouped_forward", &w4a16_grouped_forward, "The same product with one 4-bit matrix per expert.", py::arg("x"), py::arg("plane"),
+          py::arg("scales"), py::arg("zeros"), py::arg("offsets"), py::arg("rows") = py::none(), py::arg("group_size") = 128,
+          py::arg("out") = py::none());
+    m.def("moe_route", &moe_route, "Top-k experts, their weights and the order by expert.", py::arg("logits"), py::arg("top_k"),
+          py::arg("renormalize") = true);
+    m.def("moe_combine", &moe_combine, "Weighted sum of the experts' rows of each token.", py::arg("y"), py::arg("slots"), py::arg("weights"));
+    m.def("w4_row_bytes", [](int64_t K) { return bgemm_w4_row_bytes(K); });
     m.def("linear_forward_cuda", &fp6_not_provided, "FP6 GEMM of the reference: not provided.");
     m.def("weight_dequant_cpu", &fp6_not_provided, "FP6 dequant of the reference: not provided.");
     m.def("plane_bytes", [](int64_t M, int64_t K) { return (int64_t)bgemm_plane_bytes(M, K); });

@@ -1,0 +1,113 @@
+// 4-bit weight format shared by the w4 kernels: element access, conversions, the rounding rules.
+//
+// A row of K codes is stored in blocks of 128 columns = 64 bytes = sixteen little-endian 32-bit words; word 4 t + w of a
+// block holds columns 32 w + 8 t + i (i = 0..7), column i in nibble i / 2 (even i) or 4 + i / 2 (odd i). So
+//   * (word >> 4 p) & 0x000f000f is the column pair (2 p, 2 p + 1) as two 16-bit fields: the pair order that both
+//     mma.sync fragments and tensor-memory operands want, without a byte permute;
+//   * the 16 bytes that thread t of a quad loads hold one word of every 32-column group, so an mma.sync of the quad stays
+//     inside one scale group for every group size (32, 64, 128).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "../../include/bgemm_b200.h"
+
+namespace bgemm {
+
+constexpr int kW4Block = 128;                    // columns per storage block
+constexpr int kW4BlockBytes = 64;
+
+template <typename T>
+struct W4Type;
+template <>
+struct W4Type<__half> {
+    using T2 = __half2;
+    static constexpr uint32_t kOnes = 0x3C003C00u;
+    static constexpr uint32_t kMagic = 0x64006400u;      // 1024 + q: the ulp of [1024, 2048) is 1
+    static constexpr float kMagicValue = 1024.f;
+    static __device__ __forceinline__ float to_float(uint16_t b) { return __half2float(__ushort_as_half(b)); }
+    static __device__ __forceinline__ uint16_t from_float(float v) { return __half_as_ushort(__float2half_rn(v)); }
+    static __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack2(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+};
+template <>
+struct W4Type<__nv_bfloat16> {
+    using T2 = __nv_bfloat162;
+    static constexpr uint32_t kOnes = 0x3F803F80u;
+    static constexpr uint32_t kMagic = 0x43004300u;      // 128 + q: the ulp of [128, 256) is 1
+    static constexpr float kMagicValue = 128.f;
+    static __device__ __forceinline__ float to_float(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
+    static __device__ __forceinline__ uint16_t from_float(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
+    static __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack2(uint32_t v) {
+        return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+    }
+};
+
+// Two values (q - z) * s, each rounded ONCE to 16 bits: the magic number turns the 4-bit fields into exact 16-bit floats
+// (magic + q), the subtraction of (magic + z) is exact (|q - z| <= 15), the product rounds.
+template <typename T>
+__device__ __forceinline__ uint32_t w4_pair(uint32_t word_shifted, typename W4Type<T>::T2 magic_zero, typename W4Type<T>::T2 scale) {
+    uint32_t v = (word_shifted & 0x000f000fu) | W4Type<T>::kMagic;
+    typename W4Type<T>::T2 h = *reinterpret_cast<typename W4Type<T>::T2*>(&v);
+    h = __hmul2(__hsub2(h, magic_zero), scale);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ typename W4Type<T>::T2 w4_splat(uint32_t bits16) {
+    uint32_t v = bits16 | (bits16 << 16);
+    return *reinterpret_cast<typename W4Type<T>::T2*>(&v);
+}
+// 16-bit pattern of magic + z, z in 0..15
+template <typename T>
+__device__ __forceinline__ uint32_t w4_magic_zero_bits(uint32_t z) { return (W4Type<T>::kMagic & 0xffffu) + (z & 15u); }
+
+// ---- launches (w4_quant.cu, w4_stream.cu, moe.cu) -----------------------------------------------------------------
+struct W4Gemm {
+    const uint8_t* plane;          // [E][M][row_bytes]
+    const uint16_t* scales;        // [E][M][groups]
+    const uint8_t* zeros;          // [E][M][groups] or null (all 8)
+    const void* x;                 // [x_rows][x_ld] 16-bit
+    const int32_t* rows;           // [slots] source row of each slot, or null (slot s reads row s)
+    const int32_t* offsets;        // [E + 1], or null: one expert, all slots
+    void* out;                     // [slots][out_ld] 16-bit
+    long long row_bytes, x_ld, x_rows, out_ld, slots;
+    int E, M, K, groups, group;
+    int x_vec;                     // rows of x start on 16-byte boundaries
+};
+
+// [first, first + count) of expert e; whatever the offsets hold, the range stays inside [0, slots).
+__device__ __forceinline__ void w4_expert_range(const W4Gemm& p, int e, int& first, int& count) {
+    if (!p.offsets) {
+        first = 0;
+        count = (int)p.slots;
+        return;
+    }
+    const int n = (int)p.slots;
+    int a = p.offsets[e], b = p.offsets[e + 1];
+    a = a < 0 ? 0 : (a > n ? n : a);
+    b = b < a ? a : (b > n ? n : b);
+    first = a;
+    count = b - a;
+}
+
+int launch_w4_quantize(cudaStream_t stream, const void* src, int dtype, long long M, long long K, long long ld, int group, int symmetric,
+                       int scale_dtype, void* plane, void* scales, void* zeros, long long batch, long long batch_stride);
+int launch_w4_dequantize(cudaStream_t stream, const void* plane, long long M, long long K, int group, const void* scales, const void* zeros,
+                         int dtype, void* out);
+int launch_w4_stream(cudaStream_t stream, const W4Gemm& p, int dtype);
+int launch_moe_route(cudaStream_t stream, const void* logits, int dtype, long long T, int E, long long ld, int top_k, int renormalize,
+                     float* weights, int32_t* experts, int32_t* offsets, int32_t* rows, int32_t* slots, int32_t* workspace);
+size_t moe_route_workspace(long long T, int E);
+int launch_moe_combine(cudaStream_t stream, const void* y, int dtype, long long slots_total, long long M, long long y_ld, const int32_t* slots,
+                       const float* weights, long long T, int top_k, void* out, long long out_ld);
+
+}  // namespace bgemm

@@ -318,6 +318,68 @@ int bgemm_linear_forward_noalloc(void* stream, const void* weight_f16, const voi
                                  int64_t M, int64_t N, int64_t K, int op, int out_kind, int out_layout,
                                  const void* alpha);
 
+/* ==== 4-bit weights and expert routing =============================================================
+ * Weight-only 4-bit matrices with a scale (and a zero point) per row and group of columns, for layers that one bit is too
+ * few for, and the routing of a mixture of experts whose matrices are stored that way. No reference counterpart (its
+ * FP6 ancestor is a dense 6-bit format; the extension's `linear_forward_cuda` slot is not provided).
+ *
+ * Value of an element: w[m, k] = (q[m, k] - z[m, k / group]) * s[m, k / group], q in 0..15, z in 0..15 (`zeros` NULL: 8
+ * everywhere; only the low four bits of a stored zero point count), s fp16 or bf16. group is 32, 64 or 128; the last
+ * group of a row may be short; scales and zeros are row-major [M, ceil(K / group)].
+ *
+ * Storage: row-major, a row is bgemm_w4_row_bytes(K) = ceil(K / 128) * 64 bytes: blocks of 128 columns, sixteen
+ * little-endian 32-bit words each; word 4 t + w holds columns 32 w + 8 t + i (i = 0..7), column i of the word in nibble
+ * i / 2 (even i) or 4 + i / 2 (odd i). Codes behind column K are ignored (bgemm_w4_quantize writes zeros or z there).
+ * The plane starts on a 16-byte boundary. A stack of matrices is stored one behind the other.                          */
+int64_t bgemm_w4_row_bytes(int64_t K);
+
+/* Quantise [M, K] (leading dimension ld; fp16, bf16 or fp32; finite values) to 4 bits. r16 = rounding to scale_dtype:
+ *   symmetric != 0: s = r16(max |w| * fl(1/7)), z = 8 (`zeros` is not written and may be NULL)
+ *   symmetric == 0: lo = min(0, min w), hi = max(0, max w), s = r16((hi - lo) * fl(1/15)), z = clamp(rint(-lo / s), 0, 15)
+ *   q = clamp(rint(w / s) + z, 0, 15), ties to even, in 32-bit arithmetic; where s is 0, q = z (8 or 0).
+ * `batch` matrices, `src_batch_stride` elements apart, fill planes, scales and zeros one behind the other.             */
+int bgemm_w4_quantize(void* stream, const void* src, int src_dtype, int64_t M, int64_t K, int64_t ld, int group, int symmetric,
+                      int scale_dtype, void* plane, void* scales, uint8_t* zeros, int64_t batch, int64_t src_batch_stride);
+
+/* The values of a plane, each rounded once to `dtype` (the scales' type): out [M, K]. A stack: M = all its rows.        */
+int bgemm_w4_dequantize(void* stream, const void* plane, int64_t M, int64_t K, int group, const void* scales, const uint8_t* zeros,
+                        int dtype, void* out);
+
+/* y[n, m] = sum_k x[n, k] w[m, k]: x [N, K] (row pitch x_ld elements) and out [N, M] (row pitch out_ld) of `dtype`, which
+ * is also the scales' type; sums in 32 bits, rounded once. Any N, M, K and alignment of x.
+ * x must be finite for finite results: Inf or NaN in a row of x makes that row's results non-finite (not others').     */
+int bgemm_w4a16_gemm(void* stream, const void* plane, int64_t M, int64_t K, int group, const void* scales, const uint8_t* zeros,
+                     const void* x, int64_t x_ld, int dtype, int64_t N, void* out, int64_t out_ld);
+
+/* The same product for E experts (at most 1024): planes, scales and zeros are stacks [E, M, ..]; slot s in
+ * [offsets[e], offsets[e + 1]) is multiplied with expert e's matrix: out[s] = W_e x[rows ? rows[s] : s]. `offsets` is a
+ * device array int32 [E + 1], ascending from 0 to at most `slots`; experts may be empty; out rows behind offsets[E] are
+ * not written. `rows` (device, int32 [slots], or NULL) names the row of x [x_rows, K] a slot reads; an index outside x
+ * counts as a row of zeros. The host never reads offsets or rows; whatever they hold, no access leaves the buffers.    */
+int bgemm_w4a16_grouped_gemm(void* stream, const void* plane, int64_t E, int64_t M, int64_t K, int group, const void* scales,
+                             const uint8_t* zeros, const void* x, int64_t x_rows, int64_t x_ld, int dtype, const int32_t* offsets,
+                             const int32_t* rows, int64_t slots, void* out, int64_t out_ld);
+
+/* Routing: for each of T tokens the top_k (at most 32, at most E) largest of its E logits (fp16, bf16 or fp32; row pitch ld).
+ *   experts int32 [T, top_k]  the choices, largest logit first, equal logits by ascending index. -inf and NaN are never
+ *                             chosen; a token with fewer than top_k other logits ends in -1 (padding rows: all -inf)
+ *   weights fp32 [T, top_k]   softmax of the chosen logits over all E of them, or over the chosen alone (renormalize);
+ *                             0 beside -1
+ *   offsets int32 [E + 1]     the choices sorted by expert, tokens in order: expert e's are offsets[e] .. offsets[e + 1]
+ *   rows    int32 [T * top_k] the token of each sorted choice; -1 behind offsets[E]
+ *   slots   int32 [T, top_k]  the place of each choice in that order, -1 beside -1
+ * offsets and rows are what bgemm_w4a16_grouped_gemm takes, slots and weights what bgemm_moe_combine takes.
+ * workspace: bgemm_moe_route_workspace_bytes(T, E) bytes (0 up to 128 tokens), any contents.                           */
+size_t bgemm_moe_route_workspace_bytes(int64_t T, int64_t E);
+int bgemm_moe_route(void* stream, const void* logits, int dtype, int64_t T, int64_t E, int64_t ld, int top_k, int renormalize,
+                    float* weights, int32_t* experts, int32_t* offsets, int32_t* rows, int32_t* slots, void* workspace,
+                    size_t workspace_bytes);
+
+/* out[t, m] = sum_j weights[t, j] * y[slots[t, j], m], j ascending, in 32 bits, rounded once; y [slots_total, M] and out
+ * [T, M] fp16 or bf16. A slot outside [0, slots_total) adds nothing; a token without slots gets zeros.                  */
+int bgemm_moe_combine(void* stream, const void* y, int dtype, int64_t slots_total, int64_t M, int64_t y_ld, const int32_t* slots,
+                      const float* weights, int64_t T, int top_k, void* out, int64_t out_ld);
+
 /* Every wait inside the kernels is time-bounded (about 0.2 s of SM clock). A wait that runs out makes its kernel
  * drain and exit normally and records a small positive code in a per-device status word (11-18: tile-per-CTA
  * GEMM, 21-29: persistent GEMM; the number names the barrier that was not reached); the results of that launch
