@@ -69,8 +69,10 @@ lib.bgemm_w4_row_bytes.restype = _i64
 lib.bgemm_w4_row_bytes.argtypes = [_i64]
 lib.bgemm_w4_quantize.argtypes = [_vp, _vp, _int, _i64, _i64, _i64, _int, _int, _int, _vp, _vp, _vp, _i64, _i64]
 lib.bgemm_w4_dequantize.argtypes = [_vp, _vp, _i64, _i64, _int, _vp, _vp, _int, _vp]
-lib.bgemm_w4a16_gemm.argtypes = [_vp, _vp, _i64, _i64, _int, _vp, _vp, _vp, _i64, _int, _i64, _vp, _i64]
-lib.bgemm_w4a16_grouped_gemm.argtypes = [_vp, _vp, _i64, _i64, _i64, _int, _vp, _vp, _vp, _i64, _i64, _int, _vp, _vp, _i64, _vp, _i64]
+lib.bgemm_w4a16_gemm.argtypes = [_vp, _vp, _i64, _i64, _int, _vp, _vp, _vp, _i64, _int, _i64, _vp, _i64, _vp, _sz]
+lib.bgemm_w4a16_workspace_bytes.restype = _sz
+lib.bgemm_w4a16_workspace_bytes.argtypes = [_i64, _i64, _i64, _i64]
+lib.bgemm_w4a16_grouped_gemm.argtypes = [_vp, _vp, _i64, _i64, _i64, _int, _vp, _vp, _vp, _i64, _i64, _int, _vp, _vp, _i64, _vp, _i64, _vp, _sz]
 lib.bgemm_moe_route_workspace_bytes.restype = _sz
 lib.bgemm_moe_route_workspace_bytes.argtypes = [_i64, _i64]
 lib.bgemm_moe_route.argtypes = [_vp, _vp, _int, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp, _vp, _vp, _vp, _sz]

@@ -45,6 +45,19 @@ W4Gemm problem(const void* plane, int E, int64_t M, int64_t K, int group, const 
     p.x_vec = aligned(x, 16) && (x_rows == 1 || x_ld % 8 == 0);
     return p;
 }
+
+// Up to 16 rows per matrix the product is bound by the weights' bytes and the register-fed kernel takes it; beyond, the
+// tensor cores. Rows of x off 16-byte boundaries cannot be loaded by TMA and stay on the former, whatever their number.
+bool on_tensor_cores(const W4Gemm& p) {
+    const long long experts = p.offsets ? (p.slots < p.E ? p.slots : p.E) : 1;
+    return p.x_vec && p.slots > 16 && p.slots > 8 * experts;
+}
+
+int run(cudaStream_t stream, const W4Gemm& p, int dtype, void* workspace, size_t workspace_bytes) {
+    if (!on_tensor_cores(p)) return launch_w4_stream(stream, p, dtype);
+    const size_t need = w4_umma_workspace(p);
+    return launch_w4_umma(stream, p, dtype, need && workspace && workspace_bytes >= need ? workspace : nullptr);
+}
 }  // namespace
 
 extern "C" {
@@ -73,26 +86,36 @@ int bgemm_w4_dequantize(void* stream, const void* plane, int64_t M, int64_t K, i
     return launch_w4_dequantize((cudaStream_t)stream, plane, M, K, group, scales, zeros, dtype, out);
 }
 
+size_t bgemm_w4a16_workspace_bytes(int64_t E, int64_t M, int64_t K, int64_t slots) {
+    if (E < 1 || M < 1 || K < 1 || slots < 1 || E > kMaxExperts || M > kMaxDim || K > kMaxDim || slots > kMaxSlots) return 0;
+    W4Gemm p{};
+    static const int32_t some = 0;
+    p.E = (int)E; p.M = (int)M; p.K = (int)K; p.slots = slots; p.x_vec = 1;
+    p.offsets = E > 1 ? &some : nullptr;          // only whether there are any counts here
+    return on_tensor_cores(p) ? w4_umma_workspace(p) : 0;
+}
+
 int bgemm_w4a16_gemm(void* stream, const void* plane, int64_t M, int64_t K, int group, const void* scales, const uint8_t* zeros, const void* x,
-                     int64_t x_ld, int dtype, int64_t N, void* out, int64_t out_ld) {
+                     int64_t x_ld, int dtype, int64_t N, void* out, int64_t out_ld, void* workspace, size_t workspace_bytes) {
     const int rc = check_gemm(plane, M, K, group, scales, x, x_ld, N, dtype, N, out, out_ld);
     if (rc) return rc;
     const W4Gemm p = problem(plane, 1, M, K, group, scales, zeros, x, x_ld, N, N, out, out_ld);
-    return launch_w4_stream((cudaStream_t)stream, p, dtype);
+    if (!aligned(workspace, 16)) return BGEMM_ERR_ALIGN;
+    return run((cudaStream_t)stream, p, dtype, workspace, workspace_bytes);
 }
 
 int bgemm_w4a16_grouped_gemm(void* stream, const void* plane, int64_t E, int64_t M, int64_t K, int group, const void* scales, const uint8_t* zeros,
                              const void* x, int64_t x_rows, int64_t x_ld, int dtype, const int32_t* offsets, const int32_t* rows, int64_t slots,
-                             void* out, int64_t out_ld) {
+                             void* out, int64_t out_ld, void* workspace, size_t workspace_bytes) {
     if (!offsets) return BGEMM_ERR_NULL;
     const int rc = check_gemm(plane, M, K, group, scales, x, x_ld, x_rows, dtype, slots, out, out_ld);
     if (rc) return rc;
     if (E < 1 || E > kMaxExperts || (!rows && x_rows < slots)) return BGEMM_ERR_SHAPE;
-    if (!aligned(offsets, 4) || !aligned(rows, 4)) return BGEMM_ERR_ALIGN;
+    if (!aligned(offsets, 4) || !aligned(rows, 4) || !aligned(workspace, 16)) return BGEMM_ERR_ALIGN;
     W4Gemm p = problem(plane, (int)E, M, K, group, scales, zeros, x, x_ld, x_rows, slots, out, out_ld);
     p.offsets = offsets;
     p.rows = rows;
-    return launch_w4_stream((cudaStream_t)stream, p, dtype);
+    return run((cudaStream_t)stream, p, dtype, workspace, workspace_bytes);
 }
 
 size_t bgemm_moe_route_workspace_bytes(int64_t T, int64_t E) {

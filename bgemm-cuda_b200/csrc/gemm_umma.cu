@@ -463,6 +463,16 @@ static EncodeTiledFn get_encode_fn() {
     return fn;
 }
 
+int encode_tensor_map(CUtensorMap* map, CUtensorMapDataType type, unsigned rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+                      const cuuint32_t* box, const cuuint32_t* ones, CUtensorMapSwizzle swizzle) {
+    EncodeTiledFn encode = get_encode_fn();
+    if (!encode) return BGEMM_ERR_DRIVER;
+    return encode(map, type, rank, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? BGEMM_OK
+               : BGEMM_ERR_DRIVER;
+}
+
 template <int NT, bool POW2, bool DEEP>
 static int launch_variant(cudaStream_t stream, const CUtensorMap& tmap, const GemmParams& p, dim3 grid) {
     using C = Cfg<NT, POW2, DEEP>;

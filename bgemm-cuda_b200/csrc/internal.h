@@ -2,6 +2,7 @@
 #pragma once
 #include <cstddef>
 #include <cstdint>
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -61,6 +62,9 @@ void apply_test_hooks(GemmParams& p);   // copies the process-wide test settings
 int sm_count();                   // SMs of the current device (cached)
 int gemm_tile_n(long long M, long long N, long long K, long long batch);
 int max_resident_clusters(int NT, int split, bool deep);   // clusters of `split` CTAs of gemm_kernel the device holds at once; -1: unknown
+// Encodes a tiled tensor map (element strides `ones`, L2 promotion 128 B, zero fill); BGEMM_ERR_DRIVER if that is not possible.
+int encode_tensor_map(CUtensorMap* map, CUtensorMapDataType type, unsigned rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+                      const cuuint32_t* box, const cuuint32_t* ones, CUtensorMapSwizzle swizzle);
 int launch_gemm(cudaStream_t stream, GemmParams p, const int8_t* acts, long long act_ld, long long batch);
 
 // Persistent variant (gemm_persist.cu); `tensor_map` points to the CUtensorMap of the activations.

@@ -395,6 +395,16 @@ torch::Tensor w4_dequantize(torch::Tensor plane, torch::Tensor scales, c10::opti
     return out;
 }
 
+// The tensor-core path (more than 16 product rows) loads x by TMA, whose rows start on 16-byte boundaries: a copy with such a
+// pitch where x has another one.
+torch::Tensor rows_on_16_bytes(const torch::Tensor& x, int64_t products) {
+    if (products <= 16 || (reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && (x.size(0) == 1 || x.stride(0) % 8 == 0))) return x;
+    const int64_t K = x.size(1);
+    auto copy = torch::empty({x.size(0), (K + 7) / 8 * 8}, x.options()).narrow(1, 0, K);
+    copy.copy_(x.detach());
+    return copy;
+}
+
 // x [N, K] times a 4-bit matrix -> [N, M] of x's type (which is the scales' type too).
 torch::Tensor w4a16_linear_forward(torch::Tensor x, torch::Tensor plane, torch::Tensor scales, c10::optional<torch::Tensor> zeros, int64_t group) {
     const char* where = "w4a16_linear_forward";
@@ -407,8 +417,12 @@ torch::Tensor w4a16_linear_forward(torch::Tensor x, torch::Tensor plane, torch::
     if (x.stride(1) != 1 || (N > 1 && x.stride(0) < K)) x = x.contiguous();
     auto out = torch::empty({N, M}, x.options());
     if (out.numel() == 0) return out;
+    x = rows_on_16_bytes(x, N);
+    const size_t need = bgemm_w4a16_workspace_bytes(1, M, K, N);
+    torch::Tensor ws;
+    if (need) ws = workspace(x.device(), need, false);
     check(bgemm_w4a16_gemm(stream_of(x), plane.data_ptr(), M, K, (int)group, scales.data_ptr(), zeros_ptr(zeros), x.data_ptr(), N > 1 ? x.stride(0) : K,
-                           dtype_code(x), N, out.data_ptr(), M),
+                           dtype_code(x), N, out.data_ptr(), M, need ? ws.data_ptr() : nullptr, need),
           "bgemm_w4a16_gemm");
     return out;
 }
@@ -444,9 +458,14 @@ torch::Tensor w4a16_grouped_forward(torch::Tensor x, torch::Tensor plane, torch:
         TORCH_CHECK(out.numel() == 0, where, ": x has no rows");
         return out;
     }
+    x = rows_on_16_bytes(x, slots);
+    const size_t need = bgemm_w4a16_workspace_bytes(E, M, K, slots);
+    torch::Tensor ws;
+    if (need) ws = workspace(x.device(), need, false);
     check(bgemm_w4a16_grouped_gemm(stream_of(x), plane.data_ptr(), E, M, K, (int)group, scales.data_ptr(), zeros_ptr(zeros), x.data_ptr(), x.size(0),
                                    x.size(0) > 1 ? x.stride(0) : K, dtype_code(x), offsets.data_ptr<int>(),
-                                   rows.has_value() ? rows->data_ptr<int>() : nullptr, slots, out.data_ptr(), slots > 1 ? out.stride(0) : M),
+                                   rows.has_value() ? rows->data_ptr<int>() : nullptr, slots, out.data_ptr(), slots > 1 ? out.stride(0) : M,
+                                   need ? ws.data_ptr() : nullptr, need),
           "bgemm_w4a16_grouped_gemm");
     return out;
 }

@@ -104,6 +104,8 @@ int launch_w4_quantize(cudaStream_t stream, const void* src, int dtype, long lon
 int launch_w4_dequantize(cudaStream_t stream, const void* plane, long long M, long long K, int group, const void* scales, const void* zeros,
                          int dtype, void* out);
 int launch_w4_stream(cudaStream_t stream, const W4Gemm& p, int dtype);
+size_t w4_umma_workspace(const W4Gemm& p);       // bytes of partial sums the call wants; 0: none
+int launch_w4_umma(cudaStream_t stream, const W4Gemm& p, int dtype, void* workspace);
 int launch_moe_route(cudaStream_t stream, const void* logits, int dtype, long long T, int E, long long ld, int top_k, int renormalize,
                      float* weights, int32_t* experts, int32_t* offsets, int32_t* rows, int32_t* slots, int32_t* workspace);
 size_t moe_route_workspace(long long T, int E);

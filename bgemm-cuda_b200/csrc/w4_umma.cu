@@ -1,0 +1,673 @@
+// 4-bit weights x many rows of 16-bit activations on the tensor cores, dense or grouped by expert with ragged row counts:
+// y[n, m] = sum_k x[n, k] r16((q[m, k] - z) s), 32-bit accumulators in tensor memory.
+//
+// CTA pairs (tcgen05 cta_group::2) walk over tiles of 256 weight rows x up to 256 activation rows. Each CTA streams ITS 128
+// weight rows as packed codes (TMA, 64 bytes of a row per 128 columns), unpacks them in registers and writes them to its tensor
+// memory as the A operand (".ts" form); it loads half of the activation rows (TMA, 128-byte swizzle; row by row with
+// tile::gather4 where an index names the rows), and one thread of the even CTA issues the products for both SMs. Why pairs:
+// a weight is 4 bits on its way to the SM and 16 inside, so the activations are what loads the L2 -> SM path; a pair needs
+// half a tile's activations per SM (32 bytes a clock at full tensor rate, 64 without the pair: all an SM can take in).
+// Why the weights are the M side: a tile's width in activation rows is then free (any multiple of 32), which is what ragged
+// groups need: an expert with 40 rows costs 64 columns of tensor work, not 128 or 256.
+//
+// Work: tiles are (activation tile, weight tile) pairs over all experts; every CTA derives the same list from the offsets, so
+// the host never reads them. The tile width is chosen on the device too, from the counts: the width whose number of rounds
+// over the pairs, times the time of a tile (tensor work or the weights' bytes, whichever is longer), is least.
+// Few tiles (splits > 1): K is divided, the partial sums go to a workspace as 32-bit values and a second kernel adds them up
+// in a fixed order.
+//
+// The weight is rounded once to 16 bits, because the scale changes along K and the accumulator cannot: (q - z) s has up to
+// 15 significant bits, r16 keeps 11 (8). Sums are 32-bit.
+//
+// Tensor memory: 256 accumulator columns as two halves of 128 (a tile of up to 128 rows takes one of them, so its epilogue
+// runs under the next tile's products; a wider one takes both) + 4 operand stages of 64 columns (128 weights columns each).
+//   warps 0-15   unpack: set s = warps 4 s .. takes every fourth 128-column block
+//   warps 16-23  epilogue: accumulator -> 16-bit staging tile -> 16-byte stores
+//   warp 24      tensor-memory allocation; one lane of the even CTA issues the UMMAs
+//   warp 25      one lane streams the codes
+//   warp 26      activations: one lane (boxes of 16 rows), or all lanes, four rows each (gather4)
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "internal.h"
+#include "ptx.cuh"
+#include "w4.cuh"
+
+namespace bgemm {
+
+constexpr int kUThreads = 864;
+constexpr int kUSets = 4;
+constexpr int kUWarpEpi = 16, kUWarpMma = 24, kUWarpW = 25, kUWarpB = 26;
+constexpr int kUMaxExperts = 1024;
+constexpr long long kUCopyDrainClocks = 4000000;  // ~2 ms: far beyond any TMA copy in flight
+
+struct UCfg {
+    static constexpr int NT = 256;                          // widest tile
+    static constexpr int STAGES = 4, A_STAGE_COLS = 64, A_COL0 = NT;
+    static constexpr int B_SUB_BYTES = 128 * 128;           // 64 columns of this CTA's half of the activation rows
+    static constexpr int B_STAGE_BYTES = 2 * B_SUB_BYTES;
+    static constexpr int W_STAGES = 6, W_STAGE_BYTES = 128 * kW4BlockBytes;
+    static constexpr int PITCH = 272;                       // bytes of a staged result column: 128 x 2 + 16
+    static constexpr int STAGING_BYTES = 128 * PITCH;       // 64 columns per epilogue half
+    // w_full/w_empty, full/empty, d_full[2], d_empty[2], drained
+    static constexpr int NBARS = 2 * W_STAGES + 2 * STAGES + 5;
+    static constexpr int MISC_BYTES = 512 + 2 * 4 * (kUMaxExperts + 8);
+    static constexpr int SMEM_BYTES = STAGES * B_STAGE_BYTES + W_STAGES * W_STAGE_BYTES + STAGING_BYTES + MISC_BYTES + 1024;
+    static_assert(STAGES == kUSets, "an operand stage always meets the same unpack set");
+    static_assert(NBARS * 8 <= 256, "barrier area");
+    static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
+    static_assert(SMEM_BYTES > 114 * 1024, "one CTA per SM: the tensor-memory allocation never waits");
+};
+
+struct W4UmmaParams {
+    W4Gemm g;
+    float* partial;              // [splits][slots][M] or null
+    int* status;
+    long long wait_budget;
+    int splits;
+    int mpairs;                  // tiles of 256 weight rows
+};
+
+// kind::f16, both operands K-major, 32-bit accumulator, M = 256 over the pair.
+__host__ __device__ constexpr uint32_t umma_idesc_16(bool bf16, int n) {
+    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+}
+__device__ __forceinline__ void umma_f16_ts_pair(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8, %9, %10, %11, %12}, p;\n}\n" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0), "r"(0), "r"(0), "r"(0), "r"(0)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
+        "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]),
+        "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+// Four rows of a matrix whose tensor map has boxes of one row, to consecutive rows of a swizzled tile.
+__device__ __forceinline__ void tma_gather4_pair(uint32_t dst_smem, const CUtensorMap* map, int c0, const int (&row)[4], uint32_t bar_cluster) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(
+            dst_smem),
+        "l"(map), "r"(c0), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]), "r"(bar_cluster)
+        : "memory");
+}
+
+struct UTile {
+    int expert, first, valid, n;      // slots [first, first + valid), n = valid rounded up to 32
+    int m0;                           // first weight row of the pair's tile
+    int kb0, kb1, split;              // 128-column blocks
+};
+
+// The list of tiles, derived from the offsets by every CTA alike (shared memory, read-only after the prologue).
+struct UPlan {
+    const int* first;                 // [E + 1]
+    const int* tiles;                 // [E + 1] exclusive prefix of activation tiles
+    int E, mpairs, splits, nkb;
+    __device__ __forceinline__ int total() const { return tiles[E] * mpairs * splits; }
+    __device__ __forceinline__ UTile get(int t) const {
+        UTile r;
+        r.split = t % splits;
+        t /= splits;
+        const int rt = t % mpairs, tt = t / mpairs;
+        int lo = 0, hi = E;           // tiles[lo] <= tt < tiles[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (tiles[mid] <= tt) lo = mid;
+            else hi = mid;
+        }
+        const int k = tiles[lo + 1] - tiles[lo], count = first[lo + 1] - first[lo];
+        const int step = ((count + k - 1) / k + 31) & ~31;      // the expert's rows in equal tiles
+        const int at = (tt - tiles[lo]) * step;
+        r.expert = lo;
+        r.first = first[lo] + at;
+        r.valid = count - at < step ? count - at : step;
+        r.n = (r.valid + 31) & ~31;
+        r.m0 = rt * 256;
+        r.kb0 = (int)((long long)nkb * r.split / splits);
+        r.kb1 = (int)((long long)nkb * (r.split + 1) / splits);
+        return r;
+    }
+};
+
+// Which accumulator halves a tile takes, and how often each has been used: every role steps through the same sequence.
+struct UHalves {
+    int next = 0, used[2] = {0, 0}, led[2] = {0, 0};
+    int mask, lead;                   // lead: the half whose d_full barrier announces the tile
+    __device__ __forceinline__ void take(int n) {
+        if (n > 128) {
+            mask = 3;
+            lead = 0;
+        } else {
+            mask = 1 << next;
+            lead = next;
+            next ^= 1;
+        }
+    }
+    __device__ __forceinline__ void done() {
+        if (mask & 1) used[0]++;
+        if (mask & 2) used[1]++;
+        led[lead]++;
+    }
+};
+
+template <typename T, int GW, bool GATHER>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kUThreads, 1)
+w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const W4UmmaParams p) {
+    using C = UCfg;
+    grid_launch_dependents();
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sB = smem;
+    uint8_t* sW = sB + C::STAGES * C::B_STAGE_BYTES;
+    uint8_t* sOut = sW + C::W_STAGES * C::W_STAGE_BYTES;
+    uint8_t* misc = sOut + C::STAGING_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(misc);
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(misc + 256);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+    long long* s_cost = reinterpret_cast<long long*>(misc + 320);          // [8]
+    int* s_first = reinterpret_cast<int*>(misc + 512);
+    int* s_tiles = s_first + kUMaxExperts + 8;
+
+    const uint32_t w_full = smem_u32(bars);
+    const uint32_t w_empty = w_full + 8 * C::W_STAGES;
+    const uint32_t full = w_empty + 8 * C::W_STAGES;     // [S] even CTA: operand stage filled in both CTAs
+    const uint32_t empty = full + 8 * C::STAGES;         // [S] both CTAs: operand stage consumed
+    const uint32_t d_full = empty + 8 * C::STAGES;       // [2] both CTAs: accumulator (half) complete
+    const uint32_t d_empty = d_full + 16;                // [2] even CTA: accumulator half read out in both CTAs
+    const uint32_t drained = d_empty + 16;               // both CTAs: every UMMA has been executed
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    const int cid = blockIdx.x >> 1, ncl = gridDim.x >> 1;
+    const uint32_t full_leader = mapa_shared(full, 0);
+    const uint32_t d_empty_leader = mapa_shared(d_empty, 0);
+    const int nkb = (p.g.K + kW4Block - 1) / kW4Block;
+
+    if (warp == 0) {
+        for (int i = lane; i < C::NBARS; i += 32) {
+            const int f0 = 2 * C::W_STAGES, d0 = f0 + 2 * C::STAGES;
+            int count = 1;
+            if (i >= C::W_STAGES && i < 2 * C::W_STAGES) count = 4;           // w_empty: unpack warps of a set
+            else if (i >= f0 && i < f0 + C::STAGES) count = 9;                // full: activation producer + unpack warps of a set in both CTAs
+            else if (i == d0 + 2 || i == d0 + 3) count = 16;                  // d_empty: epilogue warps of both CTAs
+            mbar_init(w_full + 8 * i, count);
+        }
+        if (lane == 0) { *abort_flag = 0; set_wait_budget(abort_flag, p.wait_budget); }
+        mbar_fence_init();
+    } else if (warp == kUWarpMma) {
+        tmem_alloc_pair(smem_u32(tmem_holder), 512);
+    } else if (warp == kUWarpB && lane == 0) {
+        tma_prefetch_desc(&tmap_x);
+        tma_prefetch_desc(&tmap_w);
+    }
+    grid_dependency_wait();
+
+    // ---- the plan: counts of the experts, tile width, prefix sums ----
+    const int E = p.g.E;
+    if (warp == 1) {
+        int carry = 0;                                   // ranges are made ascending and kept inside [0, slots]
+        for (int base = 0; base <= E; base += 32) {
+            const int e = base + lane;
+            int v = 0;
+            if (e <= E) {
+                v = p.g.offsets ? p.g.offsets[e] : (e ? (int)p.g.slots : 0);
+                v = v < 0 ? 0 : (v > (int)p.g.slots ? (int)p.g.slots : v);
+            }
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) v = max(v, __shfl_up_sync(0xffffffffu, v, d));
+            v = max(v, carry);
+            if (e <= E) s_first[e] = v;
+            carry = __shfl_sync(0xffffffffu, v, 31);
+        }
+    }
+    __syncthreads();
+    if (warp < 8) {                                      // candidate widths 32, 64 .. 256
+        const int nt = 32 * (warp + 1);
+        int tiles = 0;
+        for (int e = lane; e < E; e += 32) tiles += (s_first[e + 1] - s_first[e] + nt - 1) / nt;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, d);
+        if (lane == 0) {
+            const long long rounds = ((long long)tiles * p.mpairs * p.splits + ncl - 1) / ncl;
+            // clocks of a tile: 4 per column and 128-column block of tensor work, ~360 per block for the codes at this SM's share
+            // of the memory, and a fixed part for filling the pipeline and draining the accumulator
+            const long long per_block = 4 * nt > 360 ? 4 * nt : 360;
+            s_cost[warp] = rounds * (per_block * ((nkb + p.splits - 1) / p.splits) + 2000 + 6 * nt);
+        }
+    }
+    __syncthreads();
+    if (warp == 1) {
+        int best = 7;
+        for (int c = 6; c >= 0; c--)
+            if (s_cost[c] < s_cost[best]) best = c;
+        const int nt = 32 * (best + 1);
+        int carry = 0;
+        for (int base = 0; base < E; base += 32) {
+            const int e = base + lane;
+            const int x = e < E ? (s_first[e + 1] - s_first[e] + nt - 1) / nt : 0;
+            int s = x;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, s, d);
+                if (lane >= d) s += up;
+            }
+            if (e < E) s_tiles[e] = carry + s - x;
+            carry += __shfl_sync(0xffffffffu, s, 31);
+        }
+        if (lane == 0) s_tiles[E] = carry;
+    }
+    tc_fence_before();
+    __syncwarp();
+    // Both CTAs' barriers exist before anybody signals across the pair; the plan is visible to the CTA.
+    cluster_arrive_release();
+    cluster_wait_acquire();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_holder;
+    const uint32_t tmem_a = tmem + C::A_COL0;
+    const UPlan plan{s_first, s_tiles, E, p.mpairs, p.splits, nkb};
+    const int total = plan.total();
+
+    if (warp == kUWarpW) {
+        // ---------------- codes: this CTA's 128 rows ----------------
+        if (lane == 0) {
+            long long g = 0;
+            bool ok = true;
+            for (int t = cid; t < total && ok; t += ncl) {
+                const UTile u = plan.get(t);
+                const int row = u.m0 + (int)rank * 128;
+                for (int i = u.kb0; i < u.kb1; i++, g++) {
+                    const int s = (int)(g % C::W_STAGES);
+                    if (g >= C::W_STAGES) ok = mbar_wait_relaxed(w_empty + 8 * s, (uint32_t)((g / C::W_STAGES) - 1) & 1, abort_flag, p.status, 51);
+                    if (!ok) break;
+                    mbar_arrive_expect_tx(w_full + 8 * s, C::W_STAGE_BYTES);
+                    tma_load_3d(smem_u32(sW + s * C::W_STAGE_BYTES), &tmap_w, i * kW4BlockBytes, row, u.expert, w_full + 8 * s);
+                }
+            }
+            if (*abort_flag) {  // drain own copies before the CTA may exit
+                for (long long i = g - 1; i >= 0 && i >= g - C::W_STAGES; i--) {
+                    const long long t0 = clock64();
+                    while (!mbar_test(w_full + 8 * (int)(i % C::W_STAGES), (uint32_t)(i / C::W_STAGES) & 1) && clock64() - t0 < wait_budget_of(abort_flag)) {}
+                }
+            }
+        }
+    } else if (warp == kUWarpB) {
+        // ---------------- activations: this CTA's half of the tile's rows ----------------
+        long long g = 0;
+        bool ok = true;
+        for (int t = cid; t < total && ok; t += ncl) {
+            const UTile u = plan.get(t);
+            const int half = u.n >> 1;                               // a multiple of 16
+            const int at = (int)rank * half;
+            int row[4] = {0, 0, 0, 0};
+            if (GATHER) {
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const int n = at + lane * 4 + q;
+                    // rows behind the tile and indices outside x lie outside the tensor map: zeros
+                    int r = -1;
+                    if (lane * 4 < half && n < u.valid) r = p.g.rows[u.first + n];
+                    row[q] = r < 0 || r >= (int)p.g.x_rows ? (int)p.g.x_rows : r;
+                }
+            }
+            for (int i = u.kb0; i < u.kb1; i++, g++) {
+                const int s = (int)(g % C::STAGES);
+                if (GATHER || lane == 0) {
+                    if (g >= C::STAGES) ok = mbar_wait_relaxed(empty + 8 * s, (uint32_t)((g / C::STAGES) - 1) & 1, abort_flag, p.status, 52);
+                }
+                if (GATHER) ok = __all_sync(0xffffffffu, ok);
+                else ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+                if (!ok) break;
+                // one arrival for the pair, announcing the bytes of both halves
+                if (lane == 0 && leader) mbar_arrive_expect_tx(full + 8 * s, 2 * half * 256);
+                __syncwarp();
+                const uint32_t dst = smem_u32(sB + s * C::B_STAGE_BYTES);
+                if (GATHER) {
+                    if (lane * 4 < half) {
+                        tma_gather4_pair(dst + lane * 512, &tmap_x, i * kW4Block, row, full_leader + 8 * s);
+                        tma_gather4_pair(dst + C::B_SUB_BYTES + lane * 512, &tmap_x, i * kW4Block + 64, row, full_leader + 8 * s);
+                    }
+                } else if (lane == 0) {
+                    for (int r = 0; r < half; r += 16) {
+                        tma_load_3d_pair(dst + r * 128, &tmap_x, i * kW4Block, u.first + at + r, 0, full_leader + 8 * s);
+                        tma_load_3d_pair(dst + C::B_SUB_BYTES + r * 128, &tmap_x, i * kW4Block + 64, u.first + at + r, 0, full_leader + 8 * s);
+                    }
+                }
+            }
+        }
+        if (*abort_flag) {
+            // The copies in flight must land before the CTA may exit. Their barrier also needs the unpack warps, which have
+            // stopped: wait for the longest plausible copy time instead of the barrier.
+            const long long t0 = clock64();
+            while (g > 0 && clock64() - t0 < kUCopyDrainClocks) {}
+        }
+    } else if (warp == kUWarpMma) {
+        // ---------------- UMMA issuer (even CTA) ----------------
+        if (lane == 0 && leader) {
+            bool ok = true;
+            long long g = 0;
+            UHalves h;
+            for (int t = cid; t < total && ok; t += ncl) {
+                const UTile u = plan.get(t);
+                h.take(u.n);
+                // the first product of a tile overwrites its accumulator: the epilogue warps of both CTAs must have read it out
+                if ((h.mask & 1) && h.used[0] > 0) ok = mbar_wait(d_empty, (uint32_t)(h.used[0] - 1) & 1, abort_flag, p.status, 55);
+                if (ok && (h.mask & 2) && h.used[1] > 0) ok = mbar_wait(d_empty + 8, (uint32_t)(h.used[1] - 1) & 1, abort_flag, p.status, 55);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t idesc = umma_idesc_16(W4Type<T>::kMagicValue == 128.f, u.n);
+                const uint32_t d = tmem + h.lead * 128;
+                for (int i = u.kb0; i < u.kb1; i++, g++) {
+                    const int s = (int)(g % C::STAGES);
+                    ok = mbar_wait(full + 8 * s, (uint32_t)(g / C::STAGES) & 1, abort_flag, p.status, 53);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t bbase = smem_u32(sB + s * C::B_STAGE_BYTES);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const uint64_t bdesc = umma_desc_sw128(bbase + (j >> 2) * C::B_SUB_BYTES + (j & 3) * 32);
+                        umma_f16_ts_pair(d, tmem_a + s * C::A_STAGE_COLS + j * 8, bdesc, idesc, (i > u.kb0 || j) ? 1u : 0u);
+                    }
+                    umma_commit_pair_mask(empty + 8 * s, (uint16_t)3);
+                }
+                if (!ok) break;
+                umma_commit_pair_mask(d_full + 8 * h.lead, (uint16_t)3);
+                h.done();
+            }
+            umma_commit_pair_mask(drained, (uint16_t)3);
+        }
+    } else if (warp < 4 * kUSets) {
+        // ---------------- unpack: set s takes the blocks g of the CTA's stream with g % 4 == s ----------------
+        const int set = warp >> 2;
+        const int r = (warp & 3) * 32 + lane;                 // weight row of this CTA's half tile == tensor-memory lane
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+        constexpr int G = 4 / GW;                             // scale groups of a block
+        bool ok = true;
+        long long g0 = 0;                                     // first block number of the tile
+        for (int t = cid; t < total && ok; t += ncl) {
+            const UTile u = plan.get(t);
+            int m = u.m0 + (int)rank * 128 + r;
+            if (m >= p.g.M) m = p.g.M - 1;                    // rows behind the matrix: zero codes from the tensor map, any scale
+            const long long at = ((long long)u.expert * p.g.M + m) * p.g.groups;
+            const uint16_t* srow = p.g.scales + at;
+            const uint8_t* zrow = p.g.zeros ? p.g.zeros + at : nullptr;
+            uint32_t sc[G], ze[G];
+            auto fetch = [&](int kb) {
+#pragma unroll
+                for (int q = 0; q < G; q++) {
+                    int grp = kb * G + q;
+                    if (grp >= p.g.groups) grp = p.g.groups - 1;      // behind K: the activations there are zero
+                    sc[q] = __ldg(srow + grp);
+                    ze[q] = zrow ? __ldg(zrow + grp) : 8u;
+                }
+            };
+            int kb = u.kb0 + (int)((set - g0) & 3);
+            if (kb < u.kb1) fetch(kb);
+            for (; kb < u.kb1 && ok; kb += kUSets) {
+                const long long g = g0 + (kb - u.kb0);
+                const int ws = (int)(g % C::W_STAGES);
+                ok = mbar_wait(w_full + 8 * ws, (uint32_t)(g / C::W_STAGES) & 1, abort_flag, p.status, 57);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                // TMA's 64-byte swizzle: 16-byte piece c of row r sits at piece c ^ (r / 2 % 4)
+                const uint8_t* src = sW + ws * C::W_STAGE_BYTES + r * kW4BlockBytes;
+                const int x = (r >> 1) & 3;
+                const uint4 c0 = *reinterpret_cast<const uint4*>(src + ((0 ^ x) << 4));
+                const uint4 c1 = *reinterpret_cast<const uint4*>(src + ((1 ^ x) << 4));
+                const uint4 c2 = *reinterpret_cast<const uint4*>(src + ((2 ^ x) << 4));
+                const uint4 c3 = *reinterpret_cast<const uint4*>(src + ((3 ^ x) << 4));
+                fence_proxy_async_smem();     // generic-proxy reads before the producer's next copy into this stage
+                __syncwarp();
+                if (lane == 0) mbar_arrive(w_empty + 8 * ws);
+                uint32_t s_now[G], z_now[G];
+#pragma unroll
+                for (int q = 0; q < G; q++) { s_now[q] = sc[q]; z_now[q] = ze[q]; }
+                if (kb + kUSets < u.kb1) fetch(kb + kUSets);
+                const int as = (int)(g % C::STAGES);
+                if (g >= C::STAGES) ok = mbar_wait_relaxed(empty + 8 * as, (uint32_t)((g / C::STAGES) - 1) & 1, abort_flag, p.status, 58);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    const auto s2 = w4_splat<T>(s_now[w / GW]);
+                    const auto mz = w4_splat<T>(w4_magic_zero_bits<T>(z_now[w / GW]));
+                    const uint32_t word[4] = {w == 0 ? c0.x : (w == 1 ? c0.y : (w == 2 ? c0.z : c0.w)), w == 0 ? c1.x : (w == 1 ? c1.y : (w == 2 ? c1.z : c1.w)),
+                                              w == 0 ? c2.x : (w == 1 ? c2.y : (w == 2 ? c2.z : c2.w)), w == 0 ? c3.x : (w == 1 ? c3.y : (w == 2 ? c3.z : c3.w))};
+                    uint32_t v[16];
+#pragma unroll
+                    for (int q = 0; q < 16; q++) v[q] = w4_pair<T>(word[q >> 2] >> (4 * (q & 3)), mz, s2);
+                    tmem_st16(tmem_a + lane_base + as * C::A_STAGE_COLS + w * 16, v);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(full_leader + 8 * as);
+            }
+            g0 += u.kb1 - u.kb0;
+        }
+    } else if (warp >= kUWarpEpi && warp < kUWarpEpi + 8) {
+        // ---------------- epilogue: this CTA's 128 weight rows; columns [hw n / 2, (hw + 1) n / 2) per group of four warps ----------------
+        const int hw = (warp - kUWarpEpi) >> 2;
+        const int et = (warp & 3) * 32 + lane;                // weight row == tensor-memory lane; also the thread's number in its group
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+        uint8_t* stage = sOut + hw * 64 * C::PITCH;
+        const bool vec = p.g.out_ld % 8 == 0 && (reinterpret_cast<uintptr_t>(p.g.out) & 15) == 0;
+        UHalves h;
+        for (int t = cid; t < total; t += ncl) {
+            const UTile u = plan.get(t);
+            h.take(u.n);
+            bool ok = mbar_wait_relaxed(d_full + 8 * h.lead, (uint32_t)h.led[h.lead] & 1, abort_flag, p.status, 59);
+            if (named_bar_or(1 + hw, 128, !ok)) break;        // one answer for the four warps
+            tc_fence_after();
+            const int ncols = u.n >> 1, col0 = hw * ncols;    // a multiple of 16
+            const uint32_t acc = tmem + h.lead * 128 + lane_base + col0;
+            const int m0 = u.m0 + (int)rank * 128;
+            for (int c0 = 0; c0 < ncols; c0 += 64) {
+                const int nc = ncols - c0 < 64 ? ncols - c0 : 64;
+                if (c0) named_bar_sync(1 + hw, 128);          // the staging columns have been stored
+                for (int c = 0; c < nc; c += 16) {
+                    uint32_t v[16];
+                    tmem_ld16(acc + c0 + c, v);
+                    tmem_wait_ld();
+                    if (p.partial) {
+#pragma unroll
+                        for (int q = 0; q < 16; q++) {
+                            const int n = col0 + c0 + c + q;
+                            if (n < u.valid && m0 + et < p.g.M)
+                                p.partial[((long long)u.split * p.g.slots + u.first + n) * p.g.M + m0 + et] = __uint_as_float(v[q]);
+                        }
+                        __syncwarp();
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 16; q++)
+                            *reinterpret_cast<uint16_t*>(stage + (c + q) * C::PITCH + et * 2) = W4Type<T>::from_float(__uint_as_float(v[q]));
+                    }
+                }
+                if (c0 + 64 >= ncols) {                       // everything is out of the accumulator
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (h.mask & 1) mbar_arrive_cluster(d_empty_leader);
+                        if (h.mask & 2) mbar_arrive_cluster(d_empty_leader + 8);
+                    }
+                }
+                if (!p.partial) {
+                    named_bar_sync(1 + hw, 128);
+                    // sixteen threads store the 128 rows of a column: 256 contiguous bytes
+                    for (int o = et; o < nc * 16; o += 128) {
+                        const int c = o >> 4, m = (o & 15) * 8, n = col0 + c0 + c;
+                        if (n < u.valid && m0 + m < p.g.M) {
+                            uint16_t* dst = static_cast<uint16_t*>(p.g.out) + (long long)(u.first + n) * p.g.out_ld + m0 + m;
+                            const uint4 v = *reinterpret_cast<const uint4*>(stage + c * C::PITCH + m * 2);
+                            if (vec && m0 + m + 8 <= p.g.M) {
+                                *reinterpret_cast<uint4*>(dst) = v;
+                            } else {
+                                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                                for (int q = 0; q < 8; q++)
+                                    if (m0 + m + q < p.g.M) dst[q] = (uint16_t)(w[q >> 1] >> (16 * (q & 1)));
+                            }
+                        }
+                    }
+                }
+            }
+            h.done();
+            named_bar_sync(1 + hw, 128);                      // the staging columns are free for the next tile
+        }
+    }
+    tc_fence_before();
+    __syncwarp();
+    // Both CTAs are done with each other's barriers and tensor memory before either frees it or exits.
+    cluster_arrive_release();
+    cluster_wait_acquire();
+    if (warp == kUWarpMma) {
+        if (lane == 0) {   // every UMMA has been executed before the columns are freed (immediate unless a wait ran out)
+            const long long t0 = clock64();
+            while (!mbar_test(drained, 0) && clock64() - t0 < wait_budget_of(abort_flag)) {}
+        }
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc_pair(tmem, 512);
+    }
+}
+
+// out[s, m] = r16(sum over the K partitions, in order), for the slots below offsets[E].
+template <typename T>
+__global__ void __launch_bounds__(256) w4_sum_kernel(const W4Gemm g, const float* __restrict__ partial, int splits) {
+    grid_dependency_wait();
+    long long slots = g.slots;
+    if (g.offsets) {
+        int last = 0;                                         // the largest offset: the ranges are made ascending by the product kernel
+        for (int e = threadIdx.x & 31; e <= g.E; e += 32) last = max(last, g.offsets[e]);
+        last = __reduce_max_sync(0xffffffffu, last);
+        if (last < slots) slots = last;
+    }
+    int low = 0;
+    if (g.offsets) low = g.offsets[0] < 0 ? 0 : g.offsets[0];
+    const long long chunks = (g.M + 3) / 4, total = slots * chunks;
+    const bool vec = g.M % 4 == 0;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+        const long long s = i / chunks;
+        const int m = (int)(i - s * chunks) * 4;
+        if (s < low) continue;
+        float a[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int q = 0; q < splits; q++) {
+            const float* src = partial + ((long long)q * g.slots + s) * g.M + m;
+            if (vec) {
+                const float4 v = __ldcs(reinterpret_cast<const float4*>(src));
+                a[0] += v.x; a[1] += v.y; a[2] += v.z; a[3] += v.w;
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    if (m + c < g.M) a[c] += src[c];
+            }
+        }
+        uint16_t* dst = static_cast<uint16_t*>(g.out) + s * g.out_ld + m;
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+            if (m + c < g.M) dst[c] = W4Type<T>::from_float(a[c]);
+    }
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------
+static long long expected_pairs_tiles(const W4Gemm& p) {
+    const long long mpairs = (p.M + 255) / 256;
+    const long long experts = p.offsets ? (p.slots < p.E ? p.slots : p.E) : 1;
+    const long long cols = (p.slots + 255) / 256;
+    return mpairs * (experts > cols ? experts : cols);
+}
+
+// K partitions: enough to give every pair a tile when there are few, four 128-column blocks each at least.
+static int w4_splits(const W4Gemm& p) {
+    const long long pairs = sm_count() / 2, tiles = expected_pairs_tiles(p), nkb = (p.K + kW4Block - 1) / kW4Block;
+    long long s = tiles > 0 ? pairs / tiles : 1;
+    if (s > nkb / 4) s = nkb / 4;
+    if (s > 8) s = 8;
+    return s < 2 ? 1 : (int)s;
+}
+
+size_t w4_umma_workspace(const W4Gemm& p) {
+    const int s = w4_splits(p);
+    return s > 1 ? (size_t)s * (size_t)p.slots * (size_t)p.M * 4 : 0;
+}
+
+template <typename T, int GW, bool GATHER>
+static int umma_variant(cudaStream_t stream, const CUtensorMap& tw, const CUtensorMap& tx, const W4UmmaParams& p) {
+    using C = UCfg;
+    static bool configured[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 64 || !configured[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(w4_umma_kernel<T, GW, GATHER>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+        if (e != cudaSuccess) return (int)e;
+        if (dev < 64) configured[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(sm_count() / 2 * 2), 1, 1);
+    cfg.blockDim = dim3(kUThreads, 1, 1);
+    cfg.dynamicSmemBytes = C::SMEM_BYTES;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    if (programmatic_launch_enabled()) {
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+    }
+    cudaError_t e = cudaLaunchKernelEx(&cfg, w4_umma_kernel<T, GW, GATHER>, tw, tx, p);
+    count_launch();
+    if (e != cudaSuccess) return (int)e;
+    if (p.partial) {
+        long long blocks = (p.g.slots * ((p.g.M + 3) / 4) + 255) / 256;
+        if (blocks > (long long)sm_count() * 8) blocks = (long long)sm_count() * 8;
+        e = launch_pdl(w4_sum_kernel<T>, dim3((unsigned)blocks), dim3(256), stream, p.g, (const float*)p.partial, p.splits);
+        count_launch();
+        if (e != cudaSuccess) return (int)e;
+    }
+    return (int)cudaGetLastError();
+}
+
+template <typename T>
+static int umma_dtype(cudaStream_t stream, const CUtensorMap& tw, const CUtensorMap& tx, const W4UmmaParams& p) {
+    const int gw = p.g.group / 32;
+    if (p.g.rows) {
+        if (gw == 1) return umma_variant<T, 1, true>(stream, tw, tx, p);
+        if (gw == 2) return umma_variant<T, 2, true>(stream, tw, tx, p);
+        return umma_variant<T, 4, true>(stream, tw, tx, p);
+    }
+    if (gw == 1) return umma_variant<T, 1, false>(stream, tw, tx, p);
+    if (gw == 2) return umma_variant<T, 2, false>(stream, tw, tx, p);
+    return umma_variant<T, 4, false>(stream, tw, tx, p);
+}
+
+// TMA needs rows of x on 16-byte boundaries; the sums' workspace has to be there where K is divided.
+int launch_w4_umma(cudaStream_t stream, const W4Gemm& p, int dtype, void* workspace) {
+    W4UmmaParams q{};
+    q.g = p;
+    q.status = device_status_word();
+    q.splits = workspace ? w4_splits(p) : 1;
+    q.partial = q.splits > 1 ? static_cast<float*>(workspace) : nullptr;
+    q.mpairs = (p.M + 255) / 256;
+    CUtensorMap tw, tx;
+    const cuuint64_t wdims[3] = {(cuuint64_t)p.row_bytes, (cuuint64_t)p.M, (cuuint64_t)p.E};
+    const cuuint64_t wstrides[2] = {(cuuint64_t)p.row_bytes, (cuuint64_t)p.row_bytes * (cuuint64_t)p.M};
+    const cuuint32_t wbox[3] = {(cuuint32_t)kW4BlockBytes, 128u, 1u}, ones[3] = {1u, 1u, 1u};
+    int rc = encode_tensor_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, p.plane, wdims, wstrides, wbox, ones, CU_TENSOR_MAP_SWIZZLE_64B);
+    if (rc) return rc;
+    const cuuint64_t pitch = (cuuint64_t)(p.x_rows > 1 ? p.x_ld : (p.K + 7) / 8 * 8) * 2;
+    const cuuint64_t xdims[3] = {(cuuint64_t)p.K, (cuuint64_t)p.x_rows, 1u}, xstrides[2] = {pitch, pitch * (cuuint64_t)p.x_rows};
+    const cuuint32_t xbox[3] = {64u, p.rows ? 1u : 16u, 1u};
+    const CUtensorMapDataType kind = dtype == BGEMM_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    rc = encode_tensor_map(&tx, kind, p.rows ? 2 : 3, p.x, xdims, xstrides, xbox, ones, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+    GemmParams hooks{};
+    apply_test_hooks(hooks);
+    q.wait_budget = hooks.wait_budget;
+    return dtype == BGEMM_DT_F16 ? umma_dtype<__half>(stream, tw, tx, q) : umma_dtype<__nv_bfloat16>(stream, tw, tx, q);
+}
+
+}  // namespace bgemm

@@ -347,18 +347,25 @@ int bgemm_w4_dequantize(void* stream, const void* plane, int64_t M, int64_t K, i
 
 /* y[n, m] = sum_k x[n, k] w[m, k]: x [N, K] (row pitch x_ld elements) and out [N, M] (row pitch out_ld) of `dtype`, which
  * is also the scales' type; sums in 32 bits, rounded once. Any N, M, K and alignment of x.
+ * Up to 16 rows the weights enter as the exact products above; beyond (with rows of x on 16-byte boundaries; others take
+ * the first path at any N, more slowly) each weight is first rounded to the 16-bit type, as bgemm_w4_dequantize returns it.
+ * workspace: optional, bgemm_w4a16_workspace_bytes(1, M, K, N) bytes of any contents, 16-byte aligned: partial sums of
+ * launches that have too few tiles to fill the GPU and divide K. Without it (or with less) K is not divided.
  * x must be finite for finite results: Inf or NaN in a row of x makes that row's results non-finite (not others').     */
+size_t bgemm_w4a16_workspace_bytes(int64_t E, int64_t M, int64_t K, int64_t slots);
 int bgemm_w4a16_gemm(void* stream, const void* plane, int64_t M, int64_t K, int group, const void* scales, const uint8_t* zeros,
-                     const void* x, int64_t x_ld, int dtype, int64_t N, void* out, int64_t out_ld);
+                     const void* x, int64_t x_ld, int dtype, int64_t N, void* out, int64_t out_ld, void* workspace,
+                     size_t workspace_bytes);
 
 /* The same product for E experts (at most 1024): planes, scales and zeros are stacks [E, M, ..]; slot s in
  * [offsets[e], offsets[e + 1]) is multiplied with expert e's matrix: out[s] = W_e x[rows ? rows[s] : s]. `offsets` is a
  * device array int32 [E + 1], ascending from 0 to at most `slots`; experts may be empty; out rows behind offsets[E] are
  * not written. `rows` (device, int32 [slots], or NULL) names the row of x [x_rows, K] a slot reads; an index outside x
- * counts as a row of zeros. The host never reads offsets or rows; whatever they hold, no access leaves the buffers.    */
+ * counts as a row of zeros. workspace as above, bgemm_w4a16_workspace_bytes(E, M, K, slots). The host never reads offsets or rows; whatever they hold, no access leaves the buffers.    */
 int bgemm_w4a16_grouped_gemm(void* stream, const void* plane, int64_t E, int64_t M, int64_t K, int group, const void* scales,
                              const uint8_t* zeros, const void* x, int64_t x_rows, int64_t x_ld, int dtype, const int32_t* offsets,
-                             const int32_t* rows, int64_t slots, void* out, int64_t out_ld);
+                             const int32_t* rows, int64_t slots, void* out, int64_t out_ld, void* workspace,
+                             size_t workspace_bytes);
 
 /* Routing: for each of T tokens the top_k (at most 32, at most E) largest of its E logits (fp16, bf16 or fp32; row pitch ld).
  *   experts int32 [T, top_k]  the choices, largest logit first, equal logits by ascending index. -inf and NaN are never
