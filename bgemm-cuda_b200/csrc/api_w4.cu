@@ -100,7 +100,7 @@ int bgemm_w4a16_gemm(void* stream, const void* plane, int64_t M, int64_t K, int 
     const int rc = check_gemm(plane, M, K, group, scales, x, x_ld, N, dtype, N, out, out_ld);
     if (rc) return rc;
     const W4Gemm p = problem(plane, 1, M, K, group, scales, zeros, x, x_ld, N, N, out, out_ld);
-    if (!aligned(workspace, 16)) return BGEMM_ERR_ALIGN;
+    if (!aligned(workspace, 256)) return BGEMM_ERR_ALIGN;
     return run((cudaStream_t)stream, p, dtype, workspace, workspace_bytes);
 }
 
@@ -111,7 +111,7 @@ int bgemm_w4a16_grouped_gemm(void* stream, const void* plane, int64_t E, int64_t
     const int rc = check_gemm(plane, M, K, group, scales, x, x_ld, x_rows, dtype, slots, out, out_ld);
     if (rc) return rc;
     if (E < 1 || E > kMaxExperts || (!rows && x_rows < slots)) return BGEMM_ERR_SHAPE;
-    if (!aligned(offsets, 4) || !aligned(rows, 4) || !aligned(workspace, 16)) return BGEMM_ERR_ALIGN;
+    if (!aligned(offsets, 4) || !aligned(rows, 4) || !aligned(workspace, 256)) return BGEMM_ERR_ALIGN;
     W4Gemm p = problem(plane, (int)E, M, K, group, scales, zeros, x, x_ld, x_rows, slots, out, out_ld);
     p.offsets = offsets;
     p.rows = rows;

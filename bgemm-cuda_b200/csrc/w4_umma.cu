@@ -20,12 +20,12 @@
 // 15 significant bits, r16 keeps 11 (8). Sums are 32-bit.
 //
 // Tensor memory: 256 accumulator columns as two halves of 128 (a tile of up to 128 rows takes one of them, so its epilogue
-// runs under the next tile's products; a wider one takes both) + 4 operand stages of 64 columns (128 weights columns each).
+// runs under the next tile's products; a wider one takes both) + 4 operand stages of 64 columns (128 weight columns each).
 //   warps 0-15   unpack: set s = warps 4 s .. takes every fourth 128-column block
 //   warps 16-23  epilogue: accumulator -> 16-bit staging tile -> 16-byte stores
 //   warp 24      tensor-memory allocation; one lane of the even CTA issues the UMMAs
 //   warp 25      one lane streams the codes
-//   warp 26      activations: one lane (boxes of 16 rows), or all lanes, four rows each (gather4)
+//   warps 26-27  activations, every second operand stage each: boxes of 16 to 128 rows, or four rows at a time (gather4)
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -35,7 +35,7 @@
 
 namespace bgemm {
 
-constexpr int kUThreads = 864;
+constexpr int kUThreads = 896;
 constexpr int kUSets = 4;
 constexpr int kUWarpEpi = 16, kUWarpMma = 24, kUWarpW = 25, kUWarpB = 26;
 constexpr int kUMaxExperts = 1024;
@@ -43,6 +43,9 @@ constexpr long long kUCopyDrainClocks = 4000000;  // ~2 ms: far beyond any TMA c
 
 struct UCfg {
     static constexpr int NT = 256;                          // widest tile
+    // An operand stage is 128 weight columns: 64 columns of tensor memory and 256 bytes of each activation row (two swizzled
+    // tiles of 128). Unpack set s fills stage s. (Stages of 64 columns, eight of them, measured 505 against 400 ns per 128
+    // columns of a 32-row tile: a stage costs its issuer ~330 clocks before the first product.)
     static constexpr int STAGES = 4, A_STAGE_COLS = 64, A_COL0 = NT;
     static constexpr int B_SUB_BYTES = 128 * 128;           // 64 columns of this CTA's half of the activation rows
     static constexpr int B_STAGE_BYTES = 2 * B_SUB_BYTES;
@@ -54,7 +57,7 @@ struct UCfg {
     static constexpr int MISC_BYTES = 512 + 2 * 4 * (kUMaxExperts + 8);
     static constexpr int SMEM_BYTES = STAGES * B_STAGE_BYTES + W_STAGES * W_STAGE_BYTES + STAGING_BYTES + MISC_BYTES + 1024;
     static_assert(STAGES == kUSets, "an operand stage always meets the same unpack set");
-    static_assert(NBARS * 8 <= 256, "barrier area");
+    static_assert(NBARS * 8 <= 320, "barrier area");
     static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
     static_assert(SMEM_BYTES > 114 * 1024, "one CTA per SM: the tensor-memory allocation never waits");
 };
@@ -75,15 +78,28 @@ __host__ __device__ constexpr uint32_t umma_idesc_16(bool bf16, int n) {
 __device__ __forceinline__ void umma_f16_ts_pair(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8, %9, %10, %11, %12}, p;\n}\n" ::"r"(tmem_d),
-        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0), "r"(0), "r"(0), "r"(0), "r"(0)
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+// Arrival on a barrier of either CTA of the pair, without a release at cluster scope: what is handed over is tensor memory,
+// whose accesses tcgen05.wait::st / ::ld have completed before. A cluster-scope release waits for every outstanding access
+// of the thread, the prefetched scales among them: ~2300 clocks for each arrival (a set unpacked a block in 5600 clocks instead of 3300).
+__device__ __forceinline__ void arrive_pair(uint32_t bar_cluster) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r != 0;
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
-        "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]),
-        "r"(v[14]), "r"(v[15])
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
+        "%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
+        "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]),
+        "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
         : "memory");
 }
 // Four rows of a matrix whose tensor map has boxes of one row, to consecutive rows of a swizzled tile.
@@ -94,6 +110,25 @@ __device__ __forceinline__ void tma_gather4_pair(uint32_t dst_smem, const CUtens
         "l"(map), "r"(c0), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]), "r"(bar_cluster)
         : "memory");
 }
+
+// Position in a ring of N slots: slot and how often it has come round. (Divisions of a running 64-bit block number by the ring
+// sizes cost the unpack warps a fifth of their time.)
+template <int N>
+struct URing {
+    uint32_t slot = 0, lap = 0;
+    __device__ __forceinline__ void step(uint32_t by = 1) {
+        slot += by;
+        if (slot >= N) { slot -= N; lap++; }
+    }
+    __device__ __forceinline__ uint32_t full_parity() const { return lap & 1; }
+    __device__ __forceinline__ uint32_t empty_parity() const { return (lap - 1) & 1; }     // of the previous lap; waited for when lap > 0
+};
+
+// Tensor maps of the activations: boxes of 128, 64, 32 and 16 rows, of which a tile's half is put together with as few copies
+// as possible (a copy costs its issuing thread ~150 clocks whatever its size); with an index, map 0 has boxes of one row.
+struct UXMaps {
+    CUtensorMap map[4];
+};
 
 struct UTile {
     int expert, first, valid, n;      // slots [first, first + valid), n = valid rounded up to 32
@@ -155,7 +190,7 @@ struct UHalves {
 
 template <typename T, int GW, bool GATHER>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kUThreads, 1)
-w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const W4UmmaParams p) {
+w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ UXMaps tmap_x, const W4UmmaParams p) {
     using C = UCfg;
     grid_launch_dependents();
     extern __shared__ uint8_t smem_raw[];
@@ -165,9 +200,9 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
     uint8_t* sOut = sW + C::W_STAGES * C::W_STAGE_BYTES;
     uint8_t* misc = sOut + C::STAGING_BYTES;
     uint64_t* bars = reinterpret_cast<uint64_t*>(misc);
-    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(misc + 256);
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(misc + 320);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-    long long* s_cost = reinterpret_cast<long long*>(misc + 320);          // [8]
+    long long* s_cost = reinterpret_cast<long long*>(misc + 384);          // [8]
     int* s_first = reinterpret_cast<int*>(misc + 512);
     int* s_tiles = s_first + kUMaxExperts + 8;
 
@@ -201,7 +236,7 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
     } else if (warp == kUWarpMma) {
         tmem_alloc_pair(smem_u32(tmem_holder), 512);
     } else if (warp == kUWarpB && lane == 0) {
-        tma_prefetch_desc(&tmap_x);
+        tma_prefetch_desc(&tmap_x.map[0]);
         tma_prefetch_desc(&tmap_w);
     }
     grid_dependency_wait();
@@ -274,34 +309,37 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
     if (warp == kUWarpW) {
         // ---------------- codes: this CTA's 128 rows ----------------
         if (lane == 0) {
-            long long g = 0;
+            URing<C::W_STAGES> ring;
             bool ok = true;
             for (int t = cid; t < total && ok; t += ncl) {
                 const UTile u = plan.get(t);
                 const int row = u.m0 + (int)rank * 128;
-                for (int i = u.kb0; i < u.kb1; i++, g++) {
-                    const int s = (int)(g % C::W_STAGES);
-                    if (g >= C::W_STAGES) ok = mbar_wait_relaxed(w_empty + 8 * s, (uint32_t)((g / C::W_STAGES) - 1) & 1, abort_flag, p.status, 51);
+                for (int i = u.kb0; i < u.kb1; i++, ring.step()) {
+                    if (ring.lap) ok = mbar_wait_relaxed(w_empty + 8 * ring.slot, ring.empty_parity(), abort_flag, p.status, 51);
                     if (!ok) break;
-                    mbar_arrive_expect_tx(w_full + 8 * s, C::W_STAGE_BYTES);
-                    tma_load_3d(smem_u32(sW + s * C::W_STAGE_BYTES), &tmap_w, i * kW4BlockBytes, row, u.expert, w_full + 8 * s);
+                    mbar_arrive_expect_tx(w_full + 8 * ring.slot, C::W_STAGE_BYTES);
+                    tma_load_3d(smem_u32(sW) + ring.slot * C::W_STAGE_BYTES, &tmap_w, i * kW4BlockBytes, row, u.expert, w_full + 8 * ring.slot);
                 }
             }
-            if (*abort_flag) {  // drain own copies before the CTA may exit
-                for (long long i = g - 1; i >= 0 && i >= g - C::W_STAGES; i--) {
-                    const long long t0 = clock64();
-                    while (!mbar_test(w_full + 8 * (int)(i % C::W_STAGES), (uint32_t)(i / C::W_STAGES) & 1) && clock64() - t0 < wait_budget_of(abort_flag)) {}
-                }
+            if (*abort_flag) {  // copies in flight must land before the CTA may exit: wait for the longest plausible copy time
+                const long long t0 = clock64();
+                while (clock64() - t0 < kUCopyDrainClocks) {}
             }
         }
-    } else if (warp == kUWarpB) {
-        // ---------------- activations: this CTA's half of the tile's rows ----------------
-        long long g = 0;
+    } else if (warp >= kUWarpB) {
+        // ---------------- activations: this CTA's half of the tile's rows; warp 26 the even operand stages, warp 27 the odd ones ----------------
+        // A wait, the announcement and a copy cost ~600 clocks of one thread, more than a stage's products (448 for 224 rows):
+        // one warp alone held the tensor cores to 55 %. As above, the whole warp walks and one elected lane issues.
+        const int me = warp - kUWarpB;
+        URing<C::STAGES> ring;
+        ring.step(me);
+        int skip = me;
         bool ok = true;
         for (int t = cid; t < total && ok; t += ncl) {
             const UTile u = plan.get(t);
-            const int half = u.n >> 1;                               // a multiple of 16
+            const int half = __shfl_sync(0xffffffffu, u.n >> 1, 0);  // a multiple of 16
             const int at = (int)rank * half;
+            const int row0 = __shfl_sync(0xffffffffu, u.first + at, 0);
             int row[4] = {0, 0, 0, 0};
             if (GATHER) {
 #pragma unroll
@@ -313,71 +351,92 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
                     row[q] = r < 0 || r >= (int)p.g.x_rows ? (int)p.g.x_rows : r;
                 }
             }
-            for (int i = u.kb0; i < u.kb1; i++, g++) {
-                const int s = (int)(g % C::STAGES);
-                if (GATHER || lane == 0) {
-                    if (g >= C::STAGES) ok = mbar_wait_relaxed(empty + 8 * s, (uint32_t)((g / C::STAGES) - 1) & 1, abort_flag, p.status, 52);
-                }
-                if (GATHER) ok = __all_sync(0xffffffffu, ok);
-                else ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+            const int kb1 = __shfl_sync(0xffffffffu, u.kb1, 0);
+            int i = __shfl_sync(0xffffffffu, u.kb0, 0) + skip;
+            for (; i < kb1; i += 2, ring.step(2)) {
+                const uint32_t s = ring.slot;
+                ok = __all_sync(0xffffffffu, ring.lap == 0 || mbar_wait(empty + 8 * s, ring.empty_parity(), abort_flag, p.status, 52));
                 if (!ok) break;
+                const uint32_t dst = smem_u32(sB) + s * C::B_STAGE_BYTES, bar = full_leader + 8 * s;
                 // one arrival for the pair, announcing the bytes of both halves
-                if (lane == 0 && leader) mbar_arrive_expect_tx(full + 8 * s, 2 * half * 256);
+                if (leader && elect_one()) mbar_arrive_expect_tx(full + 8 * s, 2 * half * 256);
                 __syncwarp();
-                const uint32_t dst = smem_u32(sB + s * C::B_STAGE_BYTES);
                 if (GATHER) {
                     if (lane * 4 < half) {
-                        tma_gather4_pair(dst + lane * 512, &tmap_x, i * kW4Block, row, full_leader + 8 * s);
-                        tma_gather4_pair(dst + C::B_SUB_BYTES + lane * 512, &tmap_x, i * kW4Block + 64, row, full_leader + 8 * s);
+                        tma_gather4_pair(dst + lane * 512, &tmap_x.map[0], i * kW4Block, row, bar);
+                        tma_gather4_pair(dst + C::B_SUB_BYTES + lane * 512, &tmap_x.map[0], i * kW4Block + 64, row, bar);
                     }
-                } else if (lane == 0) {
-                    for (int r = 0; r < half; r += 16) {
-                        tma_load_3d_pair(dst + r * 128, &tmap_x, i * kW4Block, u.first + at + r, 0, full_leader + 8 * s);
-                        tma_load_3d_pair(dst + C::B_SUB_BYTES + r * 128, &tmap_x, i * kW4Block + 64, u.first + at + r, 0, full_leader + 8 * s);
+                } else if (elect_one()) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const uint32_t to = dst + h * C::B_SUB_BYTES;
+                        const int c = i * kW4Block + h * 64;
+                        if (half == 128) {
+                            tma_load_3d_pair(to, &tmap_x.map[0], c, row0, 0, bar);
+                        } else {
+                            if (half & 64) tma_load_3d_pair(to, &tmap_x.map[1], c, row0, 0, bar);
+                            if (half & 32) tma_load_3d_pair(to + (half & 64) * 128, &tmap_x.map[2], c, row0 + (half & 64), 0, bar);
+                            if (half & 16) tma_load_3d_pair(to + (half & 96) * 128, &tmap_x.map[3], c, row0 + (half & 96), 0, bar);
+                        }
                     }
                 }
+                __syncwarp();
             }
+            skip = i - kb1;                                   // 0 or 1 blocks into the next tile
         }
         if (*abort_flag) {
-            // The copies in flight must land before the CTA may exit. Their barrier also needs the unpack warps, which have
-            // stopped: wait for the longest plausible copy time instead of the barrier.
-            const long long t0 = clock64();
-            while (g > 0 && clock64() - t0 < kUCopyDrainClocks) {}
+            const long long t0 = clock64();       // as above
+            while (clock64() - t0 < kUCopyDrainClocks) {}
         }
     } else if (warp == kUWarpMma) {
         // ---------------- UMMA issuer (even CTA) ----------------
-        if (lane == 0 && leader) {
+        // The whole warp walks through the loop and one elected lane issues: what the instruction takes from uniform registers
+        // (descriptors, addresses) is then computed there. A loop under "if (lane == 0)" moved every operand over for each
+        // product and cost its thread ~130 clocks apiece, more than a product of 256 columns takes.
+        if (leader) {
             bool ok = true;
-            long long g = 0;
+            URing<C::STAGES> ring;
+            bool peek = false;                        // the next stage is known to be full
             UHalves h;
+            const uint32_t bdesc_hi = (uint32_t)(umma_desc_sw128(0) >> 32);
+            const uint32_t bdesc_lo = __shfl_sync(0xffffffffu, (uint32_t)umma_desc_sw128(smem_u32(sB)), 0);
+            const uint32_t a0 = __shfl_sync(0xffffffffu, tmem_a, 0), d0 = __shfl_sync(0xffffffffu, tmem, 0);
             for (int t = cid; t < total && ok; t += ncl) {
                 const UTile u = plan.get(t);
                 h.take(u.n);
                 // the first product of a tile overwrites its accumulator: the epilogue warps of both CTAs must have read it out
                 if ((h.mask & 1) && h.used[0] > 0) ok = mbar_wait(d_empty, (uint32_t)(h.used[0] - 1) & 1, abort_flag, p.status, 55);
                 if (ok && (h.mask & 2) && h.used[1] > 0) ok = mbar_wait(d_empty + 8, (uint32_t)(h.used[1] - 1) & 1, abort_flag, p.status, 55);
+                ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t idesc = umma_idesc_16(W4Type<T>::kMagicValue == 128.f, u.n);
-                const uint32_t d = tmem + h.lead * 128;
-                for (int i = u.kb0; i < u.kb1; i++, g++) {
-                    const int s = (int)(g % C::STAGES);
-                    ok = mbar_wait(full + 8 * s, (uint32_t)(g / C::STAGES) & 1, abort_flag, p.status, 53);
+                const uint32_t idesc = __shfl_sync(0xffffffffu, umma_idesc_16(W4Type<T>::kMagicValue == 128.f, u.n), 0);
+                const uint32_t d = d0 + __shfl_sync(0xffffffffu, h.lead, 0) * 128;
+                const int steps = __shfl_sync(0xffffffffu, u.kb1 - u.kb0, 0);
+                for (int i = 0; i < steps; i++) {
+                    const uint32_t s = ring.slot;
+                    if (!peek) ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * s, ring.full_parity(), abort_flag, p.status, 53));
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t bbase = smem_u32(sB + s * C::B_STAGE_BYTES);
+                    ring.step();
+                    // the next stage is asked for before this one's products are issued: a probe takes ~100 clocks to answer
+                    const bool next = mbar_test(full + 8 * ring.slot, ring.full_parity());
+                    if (elect_one()) {
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const uint64_t bdesc = umma_desc_sw128(bbase + (j >> 2) * C::B_SUB_BYTES + (j & 3) * 32);
-                        umma_f16_ts_pair(d, tmem_a + s * C::A_STAGE_COLS + j * 8, bdesc, idesc, (i > u.kb0 || j) ? 1u : 0u);
+                        for (int j = 0; j < 8; j++) {
+                            const uint64_t bdesc = ((uint64_t)bdesc_hi << 32) | (bdesc_lo + ((s * C::B_STAGE_BYTES + (j >> 2) * C::B_SUB_BYTES + (j & 3) * 32) >> 4));
+                            umma_f16_ts_pair(d, a0 + s * C::A_STAGE_COLS + j * 8, bdesc, idesc, (i | j) ? 1u : 0u);
+                        }
+                        umma_commit_pair_mask(empty + 8 * s, (uint16_t)3);
+                        if (i == steps - 1) umma_commit_pair_mask(d_full + 8 * h.lead, (uint16_t)3);
                     }
-                    umma_commit_pair_mask(empty + 8 * s, (uint16_t)3);
+                    __syncwarp();
+                    peek = __all_sync(0xffffffffu, next);
                 }
                 if (!ok) break;
-                umma_commit_pair_mask(d_full + 8 * h.lead, (uint16_t)3);
                 h.done();
             }
-            umma_commit_pair_mask(drained, (uint16_t)3);
+            if (elect_one()) umma_commit_pair_mask(drained, (uint16_t)3);
         }
     } else if (warp < 4 * kUSets) {
         // ---------------- unpack: set s takes the blocks g of the CTA's stream with g % 4 == s ----------------
@@ -386,7 +445,10 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         constexpr int G = 4 / GW;                             // scale groups of a block
         bool ok = true;
-        long long g0 = 0;                                     // first block number of the tile
+        URing<C::W_STAGES> wring;                             // of the set's next block
+        wring.step(set);
+        uint32_t lap = 0;                                     // blocks of the set so far
+        int skip = set;                                       // blocks until the set's next one, counted from the tile's first
         for (int t = cid; t < total && ok; t += ncl) {
             const UTile u = plan.get(t);
             int m = u.m0 + (int)rank * 128 + r;
@@ -404,12 +466,12 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
                     ze[q] = zrow ? __ldg(zrow + grp) : 8u;
                 }
             };
-            int kb = u.kb0 + (int)((set - g0) & 3);
+            int kb = u.kb0 + skip;
             if (kb < u.kb1) fetch(kb);
-            for (; kb < u.kb1 && ok; kb += kUSets) {
-                const long long g = g0 + (kb - u.kb0);
-                const int ws = (int)(g % C::W_STAGES);
-                ok = mbar_wait(w_full + 8 * ws, (uint32_t)(g / C::W_STAGES) & 1, abort_flag, p.status, 57);
+            for (; kb < u.kb1 && ok; kb += kUSets, lap++) {
+                const uint32_t ws = wring.slot;
+                ok = mbar_wait(w_full + 8 * ws, wring.full_parity(), abort_flag, p.status, 57);
+                wring.step(kUSets);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 // TMA's 64-byte swizzle: 16-byte piece c of row r sits at piece c ^ (r / 2 % 4)
@@ -426,28 +488,35 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
 #pragma unroll
                 for (int q = 0; q < G; q++) { s_now[q] = sc[q]; z_now[q] = ze[q]; }
                 if (kb + kUSets < u.kb1) fetch(kb + kUSets);
-                const int as = (int)(g % C::STAGES);
-                if (g >= C::STAGES) ok = mbar_wait_relaxed(empty + 8 * as, (uint32_t)((g / C::STAGES) - 1) & 1, abort_flag, p.status, 58);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tc_fence_after();
 #pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    const auto s2 = w4_splat<T>(s_now[w / GW]);
-                    const auto mz = w4_splat<T>(w4_magic_zero_bits<T>(z_now[w / GW]));
-                    const uint32_t word[4] = {w == 0 ? c0.x : (w == 1 ? c0.y : (w == 2 ? c0.z : c0.w)), w == 0 ? c1.x : (w == 1 ? c1.y : (w == 2 ? c1.z : c1.w)),
-                                              w == 0 ? c2.x : (w == 1 ? c2.y : (w == 2 ? c2.z : c2.w)), w == 0 ? c3.x : (w == 1 ? c3.y : (w == 2 ? c3.z : c3.w))};
-                    uint32_t v[16];
+                for (int half = 0; half < 2; half++) {
+                    // the first half's arithmetic comes before the wait for the stage
+                    uint32_t v[32];
 #pragma unroll
-                    for (int q = 0; q < 16; q++) v[q] = w4_pair<T>(word[q >> 2] >> (4 * (q & 3)), mz, s2);
-                    tmem_st16(tmem_a + lane_base + as * C::A_STAGE_COLS + w * 16, v);
+                    for (int q = 0; q < 2; q++) {
+                        const int w = 2 * half + q;
+                        const auto s2 = w4_splat<T>(s_now[w / GW]);
+                        const auto mz = w4_splat<T>(w4_magic_zero_bits<T>(z_now[w / GW]));
+                        const uint32_t word[4] = {w == 0 ? c0.x : (w == 1 ? c0.y : (w == 2 ? c0.z : c0.w)), w == 0 ? c1.x : (w == 1 ? c1.y : (w == 2 ? c1.z : c1.w)),
+                                                  w == 0 ? c2.x : (w == 1 ? c2.y : (w == 2 ? c2.z : c2.w)), w == 0 ? c3.x : (w == 1 ? c3.y : (w == 2 ? c3.z : c3.w))};
+#pragma unroll
+                        for (int e = 0; e < 16; e++) v[16 * q + e] = w4_pair<T>(word[e >> 2] >> (4 * (e & 3)), mz, s2);
+                    }
+                    if (half == 0) {
+                        if (lap) ok = mbar_wait(empty + 8 * set, (lap - 1) & 1, abort_flag, p.status, 58);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        tc_fence_after();
+                    }
+                    tmem_st32(tmem_a + lane_base + set * C::A_STAGE_COLS + half * 32, v);
                 }
+                if (!ok) break;
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(full_leader + 8 * as);
+                if (lane == 0) arrive_pair(full_leader + 8 * set);
             }
-            g0 += u.kb1 - u.kb0;
+            skip = kb - u.kb1;                                // 0 .. 3
         }
     } else if (warp >= kUWarpEpi && warp < kUWarpEpi + 8) {
         // ---------------- epilogue: this CTA's 128 weight rows; columns [hw n / 2, (hw + 1) n / 2) per group of four warps ----------------
@@ -491,8 +560,8 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
-                        if (h.mask & 1) mbar_arrive_cluster(d_empty_leader);
-                        if (h.mask & 2) mbar_arrive_cluster(d_empty_leader + 8);
+                        if (h.mask & 1) arrive_pair(d_empty_leader);
+                        if (h.mask & 2) arrive_pair(d_empty_leader + 8);
                     }
                 }
                 if (!p.partial) {
@@ -573,30 +642,69 @@ __global__ void __launch_bounds__(256) w4_sum_kernel(const W4Gemm g, const float
     }
 }
 
+// The rows of x that the slots name, in slot order, rows 16 bytes apart or a multiple of it; an index outside x gives zeros.
+__global__ void __launch_bounds__(256) w4_gather_kernel(const W4Gemm g, uint16_t* __restrict__ dst, long long dst_ld) {
+    grid_dependency_wait();
+    const long long chunks = dst_ld / 8, total = g.slots * chunks;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+        const long long s = i / chunks;
+        const int k = (int)(i - s * chunks) * 8, r = __ldg(g.rows + s);
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r >= 0 && r < (int)g.x_rows) {
+            const uint16_t* src = static_cast<const uint16_t*>(g.x) + (long long)r * g.x_ld + k;
+            if (k + 8 <= g.K) {
+                v = __ldg(reinterpret_cast<const uint4*>(src));      // rows of x start on 16-byte boundaries on this path
+            } else {
+                uint32_t w[4] = {0, 0, 0, 0};
+                for (int c = 0; c < 8 && k + c < g.K; c++) w[c >> 1] |= (uint32_t)__ldg(src + c) << (16 * (c & 1));
+                v = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+        *reinterpret_cast<uint4*>(dst + s * dst_ld + k) = v;
+    }
+}
+
 // ---- host side ------------------------------------------------------------------------------------------------------
-static long long expected_pairs_tiles(const W4Gemm& p) {
-    const long long mpairs = (p.M + 255) / 256;
-    const long long experts = p.offsets ? (p.slots < p.E ? p.slots : p.E) : 1;
-    const long long cols = (p.slots + 255) / 256;
-    return mpairs * (experts > cols ? experts : cols);
-}
-
-// K partitions: enough to give every pair a tile when there are few, four 128-column blocks each at least.
+// K partitions of a launch with few tiles. A 128-column block of a tile costs a pair ~0.4 us (its codes) or 0.54 us times
+// its share of 256 columns (its products); the second kernel that adds the partitions up costs ~3.5 us and its bytes.
+// (9472 x 1024 on 256 rows, 37 tiles: 11.6 us whole, 22.6 in two.)
 static int w4_splits(const W4Gemm& p) {
-    const long long pairs = sm_count() / 2, tiles = expected_pairs_tiles(p), nkb = (p.K + kW4Block - 1) / kW4Block;
-    long long s = tiles > 0 ? pairs / tiles : 1;
-    if (s > nkb / 4) s = nkb / 4;
-    if (s > 8) s = 8;
-    return s < 2 ? 1 : (int)s;
+    const long long pairs = sm_count() / 2, mpairs = (p.M + 255) / 256, nkb = (p.K + kW4Block - 1) / kW4Block;
+    const long long experts = p.offsets ? (p.slots < p.E ? p.slots : p.E) : 1;
+    const long long rows = (p.slots + experts - 1) / experts;                 // of an expert, on average
+    const long long cols = (rows + 255) / 256, width = (rows + cols - 1) / cols;
+    const long long tiles = mpairs * experts * cols;
+    if (tiles >= pairs) return 1;
+    const double block_us = width > 190 ? 0.54 * (double)width / 256.0 : 0.4;
+    int best = 1;
+    double least = 0;
+    for (int s = 1; s <= 8 && s <= nkb; s++) {
+        const long long rounds = (tiles * s + pairs - 1) / pairs;
+        const double t = (double)rounds * (double)((nkb + s - 1) / s) * block_us + (s > 1 ? 3.5 + (double)s * (double)p.slots * (double)p.M * 8.0 / 3.0e6 : 0.0);
+        if (s == 1 || t < least) {
+            best = s;
+            least = t;
+        }
+    }
+    return best;
 }
 
-size_t w4_umma_workspace(const W4Gemm& p) {
-    const int s = w4_splits(p);
-    return s > 1 ? (size_t)s * (size_t)p.slots * (size_t)p.M * 4 : 0;
+// With an index: the rows are put together first where experts have more than 24 of them. tile::gather4 costs its issuer a
+// copy for every four rows, which holds wide tiles up (8 x 14336 x 4096 on 8192 rows: 1082 us against 694; 64 x 2048 x 4096 on
+// 2048 rows: 125 against 115), while narrow ones hide it and save the launch (64 x 1001 x 2056 on 768 rows: 40.8, 39.9 in order).
+static long long w4_gathered_ld(const W4Gemm& p, bool indexed) {
+    const long long experts = p.slots < p.E ? p.slots : p.E;
+    return indexed && p.slots > 24 * experts ? (p.K + 7) / 8 * 8 : 0;
 }
+
+static size_t partial_bytes(const W4Gemm& p) {
+    const int s = w4_splits(p);
+    return s > 1 ? align_up((size_t)s * (size_t)p.slots * (size_t)p.M * 4, 256) : 0;
+}
+size_t w4_umma_workspace(const W4Gemm& p) { return partial_bytes(p) + (size_t)p.slots * (size_t)w4_gathered_ld(p, p.offsets != nullptr) * 2; }
 
 template <typename T, int GW, bool GATHER>
-static int umma_variant(cudaStream_t stream, const CUtensorMap& tw, const CUtensorMap& tx, const W4UmmaParams& p) {
+static int umma_variant(cudaStream_t stream, const CUtensorMap& tw, const UXMaps& tx, const W4UmmaParams& p) {
     using C = UCfg;
     static bool configured[64] = {};
     int dev = 0;
@@ -632,7 +740,7 @@ static int umma_variant(cudaStream_t stream, const CUtensorMap& tw, const CUtens
 }
 
 template <typename T>
-static int umma_dtype(cudaStream_t stream, const CUtensorMap& tw, const CUtensorMap& tx, const W4UmmaParams& p) {
+static int umma_dtype(cudaStream_t stream, const CUtensorMap& tw, const UXMaps& tx, const W4UmmaParams& p) {
     const int gw = p.g.group / 32;
     if (p.g.rows) {
         if (gw == 1) return umma_variant<T, 1, true>(stream, tw, tx, p);
@@ -644,15 +752,29 @@ static int umma_dtype(cudaStream_t stream, const CUtensorMap& tw, const CUtensor
     return umma_variant<T, 4, false>(stream, tw, tx, p);
 }
 
-// TMA needs rows of x on 16-byte boundaries; the sums' workspace has to be there where K is divided.
-int launch_w4_umma(cudaStream_t stream, const W4Gemm& p, int dtype, void* workspace) {
+// TMA needs rows of x on 16-byte boundaries. Without a workspace K is not divided and rows are taken by index.
+int launch_w4_umma(cudaStream_t stream, const W4Gemm& problem, int dtype, void* workspace) {
     W4UmmaParams q{};
-    q.g = p;
+    q.g = problem;
+    W4Gemm& p = q.g;
     q.status = device_status_word();
     q.splits = workspace ? w4_splits(p) : 1;
     q.partial = q.splits > 1 ? static_cast<float*>(workspace) : nullptr;
     q.mpairs = (p.M + 255) / 256;
-    CUtensorMap tw, tx;
+    if (const long long ld = p.rows && workspace ? w4_gathered_ld(p, true) : 0) {
+        uint16_t* to = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + partial_bytes(p));
+        long long blocks = (p.slots * (ld / 8) + 255) / 256;
+        if (blocks > (long long)sm_count() * 32) blocks = (long long)sm_count() * 32;
+        const cudaError_t e = launch_pdl(w4_gather_kernel, dim3((unsigned)blocks), dim3(256), stream, p, to, ld);
+        count_launch();
+        if (e != cudaSuccess) return (int)e;
+        p.x = to;
+        p.x_ld = ld;
+        p.x_rows = p.slots;
+        p.rows = nullptr;
+    }
+    CUtensorMap tw;
+    UXMaps tx{};
     const cuuint64_t wdims[3] = {(cuuint64_t)p.row_bytes, (cuuint64_t)p.M, (cuuint64_t)p.E};
     const cuuint64_t wstrides[2] = {(cuuint64_t)p.row_bytes, (cuuint64_t)p.row_bytes * (cuuint64_t)p.M};
     const cuuint32_t wbox[3] = {(cuuint32_t)kW4BlockBytes, 128u, 1u}, ones[3] = {1u, 1u, 1u};
@@ -660,10 +782,12 @@ int launch_w4_umma(cudaStream_t stream, const W4Gemm& p, int dtype, void* worksp
     if (rc) return rc;
     const cuuint64_t pitch = (cuuint64_t)(p.x_rows > 1 ? p.x_ld : (p.K + 7) / 8 * 8) * 2;
     const cuuint64_t xdims[3] = {(cuuint64_t)p.K, (cuuint64_t)p.x_rows, 1u}, xstrides[2] = {pitch, pitch * (cuuint64_t)p.x_rows};
-    const cuuint32_t xbox[3] = {64u, p.rows ? 1u : 16u, 1u};
     const CUtensorMapDataType kind = dtype == BGEMM_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    rc = encode_tensor_map(&tx, kind, p.rows ? 2 : 3, p.x, xdims, xstrides, xbox, ones, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc) return rc;
+    for (int b = 0; b < (p.rows ? 1 : 4); b++) {
+        const cuuint32_t xbox[3] = {64u, p.rows ? 1u : 128u >> b, 1u};
+        rc = encode_tensor_map(&tx.map[b], kind, p.rows ? 2 : 3, p.x, xdims, xstrides, xbox, ones, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (rc) return rc;
+    }
     GemmParams hooks{};
     apply_test_hooks(hooks);
     q.wait_budget = hooks.wait_budget;

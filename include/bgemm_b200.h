@@ -349,8 +349,9 @@ int bgemm_w4_dequantize(void* stream, const void* plane, int64_t M, int64_t K, i
  * is also the scales' type; sums in 32 bits, rounded once. Any N, M, K and alignment of x.
  * Up to 16 rows the weights enter as the exact products above; beyond (with rows of x on 16-byte boundaries; others take
  * the first path at any N, more slowly) each weight is first rounded to the 16-bit type, as bgemm_w4_dequantize returns it.
- * workspace: optional, bgemm_w4a16_workspace_bytes(1, M, K, N) bytes of any contents, 16-byte aligned: partial sums of
- * launches that have too few tiles to fill the GPU and divide K. Without it (or with less) K is not divided.
+ * workspace: optional, bgemm_w4a16_workspace_bytes(1, M, K, N) bytes of any contents, 256-byte aligned: partial sums of
+ * launches that have too few tiles to fill the GPU and divide K, and rows of x put together (grouped product, with an
+ * index). Without it (or with less) K is not divided and the rows are read by index.
  * x must be finite for finite results: Inf or NaN in a row of x makes that row's results non-finite (not others').     */
 size_t bgemm_w4a16_workspace_bytes(int64_t E, int64_t M, int64_t K, int64_t slots);
 int bgemm_w4a16_gemm(void* stream, const void* plane, int64_t M, int64_t K, int group, const void* scales, const uint8_t* zeros,

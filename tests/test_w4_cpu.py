@@ -54,14 +54,14 @@ def test_gemm_refusals(lib):
     assert gemm(plane=None) == -1 and gemm(scales=None) == -1 and gemm(x=None) == -1 and gemm(out=None) == -1
     assert gemm(dt=2) == -4 and gemm(dt=3) == -4 and gemm(group=48) == -4
     assert gemm(M=0) == -2 and gemm(N=0) == -2 and gemm(K=0) == -2 and gemm(x_ld=63) == -2 and gemm(out_ld=7) == -2 and gemm(M=(1 << 24) + 1) == -2
-    assert gemm(plane=fake + 4) == -3 and gemm(x=fake + 1) == -3 and gemm(out=fake + 1) == -3 and gemm(ws=fake + 8) == -3
+    assert gemm(plane=fake + 4) == -3 and gemm(x=fake + 1) == -3 and gemm(out=fake + 1) == -3 and gemm(ws=fake + 16) == -3
 
     def grouped(E=4, x_rows=2, slots=2, offsets=fake, rows=None, x_ld=64, ws=None):
         return lib.bgemm_w4a16_grouped_gemm(None, fake, E, 8, 64, 32, fake, None, fake, x_rows, x_ld, 0, offsets, rows, slots, fake, 8, ws, 0)
 
     assert grouped(offsets=None) == -1 and grouped(E=0) == -2 and grouped(E=1025) == -2 and grouped(slots=0) == -2 and grouped(x_rows=0) == -2
     assert grouped(x_rows=1) == -2                                        # without an index every slot needs its row
-    assert grouped(offsets=fake + 2) == -3 and grouped(rows=fake + 2) == -3 and grouped(x_ld=1) == -2 and grouped(ws=fake + 4) == -3
+    assert grouped(offsets=fake + 2) == -3 and grouped(rows=fake + 2) == -3 and grouped(x_ld=1) == -2 and grouped(ws=fake + 128) == -3
     assert lib.bgemm_w4_dequantize(None, None, 8, 64, 32, fake, None, 0, fake) == -1
     assert lib.bgemm_w4_dequantize(None, fake, 8, 64, 33, fake, None, 0, fake) == -4
     assert lib.bgemm_w4_dequantize(None, fake, 8, 64, 32, fake, None, 2, fake) == -4
