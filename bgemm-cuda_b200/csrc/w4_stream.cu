@@ -46,20 +46,28 @@ __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], uint32_t 
 }
 
 // Eight consecutive activations of one row; columns at or beyond `valid` read as zero.
-__device__ __forceinline__ uint4 load_x8(const uint16_t* row, int k0, int valid, bool vec) {
-    if (row == nullptr || valid <= 0) return make_uint4(0, 0, 0, 0);
-    if (vec && valid >= 8) return __ldg(reinterpret_cast<const uint4*>(row + k0));
+__device__ __forceinline__ uint4 load_x8(const uint16_t* at, int valid, bool vec) {
+    if (vec && valid >= 8) return __ldg(reinterpret_cast<const uint4*>(at));
     uint32_t v[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 8; i++)
-        if (i < valid) v[i >> 1] |= (uint32_t)__ldg(row + k0 + i) << (16 * (i & 1));
+        if (i < valid) v[i >> 1] |= (uint32_t)__ldg(at + i) << (16 * (i & 1));
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
+// One 128-column block of the warp's rows in flight: the codes and, packed, the block's scales and zero points of each row.
+template <int MT, int GW>
+struct W4Slot {
+    static constexpr int G = 4 / GW;                               // scale groups of a block
+    uint4 w[2 * MT];
+    uint32_t s[2 * MT][G == 4 ? 2 : 1], z[2 * MT];
+};
+
 // MT: 16-row tiles of a CTA, NTL: 8-column tiles of activation rows per pass, GW: 32-column words per scale group (1, 2, 4).
 template <typename T, int MT, int NTL, int GW>
-__global__ void __launch_bounds__(kW4Warps * 32) w4_stream_kernel(const W4Gemm p) {
-    constexpr bool kHalf = sizeof(typename W4Type<T>::T2) == 4 && W4Type<T>::kMagicValue == 1024.f;
+__global__ void __launch_bounds__(kW4Warps * 32, MT * NTL == 4 ? 1 : 2) w4_stream_kernel(const W4Gemm p) {
+    constexpr bool kHalf = W4Type<T>::kMagicValue == 1024.f;
+    constexpr int G = 4 / GW;
     __shared__ float red[kW4Warps][NTL * 8][MT * 16 + 4];
     grid_dependency_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -85,29 +93,64 @@ __global__ void __launch_bounds__(kW4Warps * 32) w4_stream_kernel(const W4Gemm p
 
     const int row0 = blockIdx.x * (MT * 16);
     const int nblocks = (p.K + kW4Block - 1) / kW4Block;
-    const uint8_t* wrow[2 * MT];
-    const uint16_t* srow[2 * MT];
-    const uint8_t* zrow[2 * MT];
+    const int full_blocks = p.x_vec ? p.K / kW4Block : 0;          // blocks whose activations are whole 16-byte pieces
+    const bool packed = p.groups % G == 0;                         // a block's scales of a row are one aligned load
+    const long long base_row = (long long)expert * p.M + row0;
+    const uint8_t* wbase = p.plane + base_row * p.row_bytes + t * 16;
+    const uint16_t* sbase = p.scales + base_row * p.groups;
+    const uint8_t* zbase = p.zeros ? p.zeros + base_row * p.groups : nullptr;
+    uint32_t woff[2 * MT], soff[2 * MT];
 #pragma unroll
     for (int r = 0; r < 2 * MT; r++) {
-        int m = row0 + r * 8 + g;
-        if (m >= p.M) m = p.M - 1;                                 // rows behind the matrix repeat the last one and are not stored
-        const long long at = (long long)expert * p.M + m;
-        wrow[r] = p.plane + at * p.row_bytes + t * 16;
-        srow[r] = p.scales + at * p.groups;
-        zrow[r] = p.zeros ? p.zeros + at * p.groups : nullptr;
+        const int m = row0 + r * 8 + g < p.M ? r * 8 + g : p.M - 1 - row0;     // rows behind the matrix repeat the last one and are not stored
+        woff[r] = (uint32_t)m * (uint32_t)p.row_bytes;
+        soff[r] = (uint32_t)m * (uint32_t)p.groups;
     }
+    auto fetch = [&](W4Slot<MT, GW>& slot, int kb) {
+        const uint8_t* at = wbase + (long long)kb * kW4BlockBytes;
+#pragma unroll
+        for (int r = 0; r < 2 * MT; r++) slot.w[r] = ld_stream(at + woff[r]);
+        const int grp = kb * G;
+#pragma unroll
+        for (int r = 0; r < 2 * MT; r++) {
+            const uint16_t* sp = sbase + soff[r] + grp;
+            const uint8_t* zp = zbase + soff[r] + grp;
+            slot.z[r] = 0x08080808u;
+            if (G == 1) {
+                slot.s[r][0] = __ldg(sp);
+                if (zbase) slot.z[r] = __ldg(zp);
+            } else if (packed) {
+                if (G == 2) {
+                    slot.s[r][0] = __ldg(reinterpret_cast<const uint32_t*>(sp));
+                    if (zbase) slot.z[r] = __ldg(reinterpret_cast<const uint16_t*>(zp));
+                } else {
+                    const uint2 v = __ldg(reinterpret_cast<const uint2*>(sp));
+                    slot.s[r][0] = v.x;
+                    slot.s[r][G == 4 ? 1 : 0] = v.y;
+                    if (zbase) slot.z[r] = __ldg(reinterpret_cast<const uint32_t*>(zp));
+                }
+            } else {                                               // groups behind K: every activation there is zero, any scale will do
+#pragma unroll
+                for (int q = 0; q < G; q++) {
+                    const int o = grp + q < p.groups ? q : p.groups - 1 - grp;
+                    const uint32_t v = __ldg(sp + o);
+                    if (q & 1) slot.s[r][q >> 1] |= v << 16;
+                    else slot.s[r][q >> 1] = v;
+                    if (zbase) slot.z[r] = (slot.z[r] & ~(255u << (8 * q))) | (uint32_t)__ldg(zp + o) << (8 * q);
+                }
+            }
+        }
+    };
 
     for (int c0 = 0; c0 < count; c0 += NTL * 8) {
         const uint16_t* xrow[NTL];
 #pragma unroll
         for (int j = 0; j < NTL; j++) {
-            const int n = c0 + j * 8 + g;
-            xrow[j] = nullptr;
-            if (n < count) {
-                const long long src = p.rows ? (long long)p.rows[first + n] : (long long)first + n;
-                if (src >= 0 && src < p.x_rows) xrow[j] = static_cast<const uint16_t*>(p.x) + src * p.x_ld;
-            }
+            // columns behind the expert's rows and rows outside x repeat a row that exists; the former are not stored, the
+            // latter stored as zeros (a column of the product sees nothing of the others)
+            const int n = c0 + j * 8 + g < count ? c0 + j * 8 + g : count - 1;
+            const long long src = p.rows ? (long long)p.rows[first + n] : (long long)first + n;
+            xrow[j] = static_cast<const uint16_t*>(p.x) + (src >= 0 && src < p.x_rows ? src : 0) * p.x_ld + t * 8;
         }
         float y[MT][NTL][4];
 #pragma unroll
@@ -117,18 +160,21 @@ __global__ void __launch_bounds__(kW4Warps * 32) w4_stream_kernel(const W4Gemm p
 #pragma unroll
                 for (int e = 0; e < 4; e++) y[i][j][e] = 0.f;
 
-        uint4 w[2 * MT];
-        if (warp < nblocks) {
+        // One block: products, then the slot is filled with the block after the next.
+        auto block = [&](W4Slot<MT, GW>& slot, int kb) {
+            uint4 b[4][NTL];
+            if (kb < full_blocks) {
 #pragma unroll
-            for (int r = 0; r < 2 * MT; r++) w[r] = ld_stream(wrow[r] + (long long)warp * kW4BlockBytes);
-        }
-        for (int kb = warp; kb < nblocks; kb += kW4Warps) {
-            uint4 cur[2 * MT];
+                for (int word = 0; word < 4; word++)
 #pragma unroll
-            for (int r = 0; r < 2 * MT; r++) cur[r] = w[r];
-            if (kb + kW4Warps < nblocks) {
+                    for (int j = 0; j < NTL; j++) b[word][j] = __ldg(reinterpret_cast<const uint4*>(xrow[j] + kb * kW4Block + word * 32));
+            } else {
 #pragma unroll
-                for (int r = 0; r < 2 * MT; r++) w[r] = ld_stream(wrow[r] + (long long)(kb + kW4Warps) * kW4BlockBytes);
+                for (int word = 0; word < 4; word++) {
+                    const int k0 = kb * kW4Block + word * 32;
+#pragma unroll
+                    for (int j = 0; j < NTL; j++) b[word][j] = load_x8(xrow[j] + k0, p.K - k0 - t * 8, p.x_vec != 0);
+                }
             }
             float acc[MT][NTL][4], acc_hi[MT][NTL][4], gs[NTL][4];
 #pragma unroll
@@ -144,20 +190,17 @@ __global__ void __launch_bounds__(kW4Warps * 32) w4_stream_kernel(const W4Gemm p
                         }
                     }
                 }
-                uint4 b[NTL];
-                const int k0 = kb * kW4Block + word * 32 + t * 8;
-#pragma unroll
-                for (int j = 0; j < NTL; j++) b[j] = load_x8(xrow[j], k0, p.K - k0, p.x_vec != 0);
 #pragma unroll
                 for (int i = 0; i < MT; i++) {
-                    const uint32_t wa = word == 0 ? cur[2 * i].x : (word == 1 ? cur[2 * i].y : (word == 2 ? cur[2 * i].z : cur[2 * i].w));
-                    const uint32_t wb = word == 0 ? cur[2 * i + 1].x : (word == 1 ? cur[2 * i + 1].y : (word == 2 ? cur[2 * i + 1].z : cur[2 * i + 1].w));
+                    const uint4 u = slot.w[2 * i], v = slot.w[2 * i + 1];
+                    const uint32_t wa = word == 0 ? u.x : (word == 1 ? u.y : (word == 2 ? u.z : u.w));
+                    const uint32_t wb = word == 0 ? v.x : (word == 1 ? v.y : (word == 2 ? v.z : v.w));
                     if (kHalf) {
                         const uint32_t ha = wa >> 8, hb = wb >> 8;
 #pragma unroll
                         for (int j = 0; j < NTL; j++) {
-                            mma16816<T>(acc[i][j], wa & 0x000f000fu, wb & 0x000f000fu, ha & 0x000f000fu, hb & 0x000f000fu, b[j].x, b[j].z);
-                            mma16816<T>(acc_hi[i][j], wa & 0x00f000f0u, wb & 0x00f000f0u, ha & 0x00f000f0u, hb & 0x00f000f0u, b[j].y, b[j].w);
+                            mma16816<T>(acc[i][j], wa & 0x000f000fu, wb & 0x000f000fu, ha & 0x000f000fu, hb & 0x000f000fu, b[word][j].x, b[word][j].z);
+                            mma16816<T>(acc_hi[i][j], wa & 0x00f000f0u, wb & 0x00f000f0u, ha & 0x00f000f0u, hb & 0x00f000f0u, b[word][j].y, b[word][j].w);
                         }
                     } else {
                         uint32_t a[4], c[4];
@@ -168,40 +211,48 @@ __global__ void __launch_bounds__(kW4Warps * 32) w4_stream_kernel(const W4Gemm p
                         }
 #pragma unroll
                         for (int j = 0; j < NTL; j++) {
-                            mma16816<T>(acc[i][j], a[0], c[0], a[1], c[1], b[j].x, b[j].y);
-                            mma16816<T>(acc_hi[i][j], a[2], c[2], a[3], c[3], b[j].z, b[j].w);
+                            mma16816<T>(acc[i][j], a[0], c[0], a[1], c[1], b[word][j].x, b[word][j].y);
+                            mma16816<T>(acc_hi[i][j], a[2], c[2], a[3], c[3], b[word][j].z, b[word][j].w);
                         }
                     }
                 }
                 constexpr uint32_t one = W4Type<T>::kOnes;
 #pragma unroll
                 for (int j = 0; j < NTL; j++) {
-                    mma16816<T>(gs[j], one, one, one, one, b[j].x, b[j].y);
-                    mma16816<T>(gs[j], one, one, one, one, b[j].z, b[j].w);
+                    mma16816<T>(gs[j], one, one, one, one, b[word][j].x, b[word][j].y);
+                    mma16816<T>(gs[j], one, one, one, one, b[word][j].z, b[word][j].w);
                 }
                 if ((word + 1) % GW == 0) {                        // the end of a scale group
-                    int grp = kb * (4 / GW) + word / GW;
-                    if (grp >= p.groups) grp = p.groups - 1;       // behind K: every activation there is zero
+                    const int q = word / GW;
 #pragma unroll
                     for (int i = 0; i < MT; i++) {
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            const float s = W4Type<T>::to_float(__ldg(srow[2 * i + h] + grp));
-                            float z = zrow[2 * i + h] ? (float)(__ldg(zrow[2 * i + h] + grp) & 15) : 8.f;
+                            const float s = W4Type<T>::to_float((uint16_t)(slot.s[2 * i + h][q >> 1] >> (16 * (q & 1))));
+                            float z = (float)((slot.z[2 * i + h] >> (8 * q)) & 15u);
                             if (!kHalf) z += W4Type<T>::kMagicValue;
 #pragma unroll
                             for (int j = 0; j < NTL; j++) {
 #pragma unroll
                                 for (int e = 0; e < 2; e++) {
-                                    const int q = 2 * h + e;
-                                    const float sum = kHalf ? fmaf(acc[i][j][q], 16777216.f, acc_hi[i][j][q] * 1048576.f) : acc[i][j][q] + acc_hi[i][j][q];
-                                    y[i][j][q] = fmaf(s, fmaf(-z, gs[j][e], sum), y[i][j][q]);
+                                    const int k = 2 * h + e;
+                                    const float sum = kHalf ? fmaf(acc[i][j][k], 16777216.f, acc_hi[i][j][k] * 1048576.f) : acc[i][j][k] + acc_hi[i][j][k];
+                                    y[i][j][k] = fmaf(s, fmaf(-z, gs[j][e], sum), y[i][j][k]);
                                 }
                             }
                         }
                     }
                 }
             }
+            if (kb + 2 * kW4Warps < nblocks) fetch(slot, kb + 2 * kW4Warps);
+        };
+        W4Slot<MT, GW> even, odd;
+        if (warp < nblocks) fetch(even, warp);
+        if (warp + kW4Warps < nblocks) fetch(odd, warp + kW4Warps);
+#pragma unroll 1
+        for (int kb = warp; kb < nblocks; kb += 2 * kW4Warps) {
+            block(even, kb);
+            if (kb + kW4Warps < nblocks) block(odd, kb + kW4Warps);
         }
         // the eight warps' sums, in a fixed order
 #pragma unroll
@@ -217,6 +268,10 @@ __global__ void __launch_bounds__(kW4Warps * 32) w4_stream_kernel(const W4Gemm p
                 float v = 0.f;
 #pragma unroll
                 for (int q = 0; q < kW4Warps; q++) v += red[q][n][m];
+                if (p.rows) {
+                    const int src = p.rows[first + c0 + n];
+                    if (src < 0 || src >= p.x_rows) v = 0.f;
+                }
                 static_cast<uint16_t*>(p.out)[(long long)(first + c0 + n) * p.out_ld + row0 + m] = W4Type<T>::from_float(v);
             }
         }
