@@ -52,11 +52,26 @@ struct W4Type<__nv_bfloat16> {
     }
 };
 
+// (v & mask) | magic in ONE logic instruction. Written as C the two constants would be two immediates, of which an
+// instruction can hold one, and the compiler splits it.
+__device__ __forceinline__ uint32_t w4_field(uint32_t v, uint32_t mask, uint32_t magic) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(magic));
+    return r;
+}
+// A constant in a register the compiler does not see through.
+__device__ __forceinline__ uint32_t w4_opaque(uint32_t v) {
+    uint32_t r;
+    asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
 // Two values (q - z) * s, each rounded ONCE to 16 bits: the magic number turns the 4-bit fields into exact 16-bit floats
 // (magic + q), the subtraction of (magic + z) is exact (|q - z| <= 15), the product rounds.
 template <typename T>
-__device__ __forceinline__ uint32_t w4_pair(uint32_t word_shifted, typename W4Type<T>::T2 magic_zero, typename W4Type<T>::T2 scale) {
-    uint32_t v = (word_shifted & 0x000f000fu) | W4Type<T>::kMagic;
+__device__ __forceinline__ uint32_t w4_pair(uint32_t word_shifted, typename W4Type<T>::T2 magic_zero, typename W4Type<T>::T2 scale,
+                                            uint32_t magic = W4Type<T>::kMagic) {
+    uint32_t v = w4_field(word_shifted, 0x000f000fu, magic);
     typename W4Type<T>::T2 h = *reinterpret_cast<typename W4Type<T>::T2*>(&v);
     h = __hmul2(__hsub2(h, magic_zero), scale);
     return *reinterpret_cast<uint32_t*>(&h);

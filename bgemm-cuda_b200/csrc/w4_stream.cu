@@ -24,9 +24,16 @@ namespace bgemm {
 
 constexpr int kW4Warps = 8;
 
-__device__ __forceinline__ uint4 ld_stream(const void* p) {
+// 16 bytes from global to shared memory, past L1, waited for by groups.
+__device__ __forceinline__ void copy16(uint32_t dst_smem, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst_smem), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
     uint4 v;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
     return v;
 }
 
@@ -55,22 +62,25 @@ __device__ __forceinline__ uint4 load_x8(const uint16_t* at, int valid, bool vec
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// One 128-column block of the warp's rows in flight: the codes and, packed, the block's scales and zero points of each row.
-template <int MT, int GW>
-struct W4Slot {
-    static constexpr int G = 4 / GW;                               // scale groups of a block
-    uint4 w[2 * MT];
-    uint32_t s[2 * MT][G == 4 ? 2 : 1], z[2 * MT];
-};
+// Columns of one pass over the scales, which wait in shared memory as pairs (scale, zero point) of the 16-bit type.
+constexpr int kW4ChunkBlocks = 64;
+constexpr int kW4Depth = 4;                                                         // blocks of a warp on their way
+template <int GW>
+__host__ __device__ constexpr int w4_pitch() { return kW4ChunkBlocks * (4 / GW) + 1; }                  // odd: the eight rows of a warp's read meet eight banks
 
 // MT: 16-row tiles of a CTA, NTL: 8-column tiles of activation rows per pass, GW: 32-column words per scale group (1, 2, 4).
 template <typename T, int MT, int NTL, int GW>
 __global__ void __launch_bounds__(kW4Warps * 32, MT * NTL == 4 ? 1 : 2) w4_stream_kernel(const W4Gemm p) {
     constexpr bool kHalf = W4Type<T>::kMagicValue == 1024.f;
-    constexpr int G = 4 / GW;
-    __shared__ float red[kW4Warps][NTL * 8][MT * 16 + 4];
+    constexpr int G = 4 / GW, PITCH = w4_pitch<GW>(), ROWS = MT * 16;
+    // Per warp a ring of blocks that every lane fills and reads back itself (no barrier anywhere near it), then the scales
+    // [ROWS][PITCH], where the warps' sums meet afterwards.
+    extern __shared__ __align__(16) uint32_t smem[];
+    uint32_t* s_sz = smem + kW4Warps * kW4Depth * (ROWS * kW4BlockBytes / 4);
+    float(*red)[NTL * 8][ROWS + 4] = reinterpret_cast<float(*)[NTL * 8][ROWS + 4]>(s_sz);
     grid_dependency_wait();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    // the shuffle tells the compiler that the warp's number is uniform: block addresses are then computed by the uniform unit
+    const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), g = lane >> 2, t = lane & 3;
 
     int expert = 0, first, count;
     if (p.offsets) {                                               // the blockIdx.y-th expert that has rows
@@ -90,54 +100,48 @@ __global__ void __launch_bounds__(kW4Warps * 32, MT * NTL == 4 ? 1 : 2) w4_strea
         if (!found) return;
     }
     w4_expert_range(p, expert, first, count);
+    expert = __shfl_sync(0xffffffffu, expert, 0);
 
-    const int row0 = blockIdx.x * (MT * 16);
+    const int row0 = blockIdx.x * ROWS;
     const int nblocks = (p.K + kW4Block - 1) / kW4Block;
     const int full_blocks = p.x_vec ? p.K / kW4Block : 0;          // blocks whose activations are whole 16-byte pieces
-    const bool packed = p.groups % G == 0;                         // a block's scales of a row are one aligned load
+    const uint32_t magic = w4_opaque(W4Type<T>::kMagic);
     const long long base_row = (long long)expert * p.M + row0;
-    const uint8_t* wbase = p.plane + base_row * p.row_bytes + t * 16;
-    const uint16_t* sbase = p.scales + base_row * p.groups;
-    const uint8_t* zbase = p.zeros ? p.zeros + base_row * p.groups : nullptr;
-    uint32_t woff[2 * MT], soff[2 * MT];
+    const uint8_t* wbase = p.plane + base_row * p.row_bytes;
+    uint32_t woff[2 * MT];
 #pragma unroll
     for (int r = 0; r < 2 * MT; r++) {
         const int m = row0 + r * 8 + g < p.M ? r * 8 + g : p.M - 1 - row0;     // rows behind the matrix repeat the last one and are not stored
-        woff[r] = (uint32_t)m * (uint32_t)p.row_bytes;
-        soff[r] = (uint32_t)m * (uint32_t)p.groups;
+        woff[r] = (uint32_t)m * (uint32_t)p.row_bytes + t * 16;
     }
-    auto fetch = [&](W4Slot<MT, GW>& slot, int kb) {
-        const uint8_t* at = wbase + (long long)kb * kW4BlockBytes;
+    const uint32_t ring = smem_u32(smem) + warp * (kW4Depth * ROWS * kW4BlockBytes) + lane * 16;
+    auto fetch = [&](int slot, int kb) {                           // a group is committed whether there is such a block or not
+        if (kb < nblocks) {
+            const uint8_t* at = wbase + (long long)kb * kW4BlockBytes;
 #pragma unroll
-        for (int r = 0; r < 2 * MT; r++) slot.w[r] = ld_stream(at + woff[r]);
-        const int grp = kb * G;
+            for (int r = 0; r < 2 * MT; r++) copy16(ring + slot * (ROWS * kW4BlockBytes) + r * 512, at + woff[r]);
+        }
+        copy_commit();
+    };
+    // scales and zero points of the blocks [kb0, kb0 + 64): coalesced along the rows
+    auto stage_scales = [&](int kb0) {
+        const int g0 = kb0 * G, n = p.groups - g0 < kW4ChunkBlocks * G ? p.groups - g0 : kW4ChunkBlocks * G;
+        const int want = (n + G - 1) / G * G;                      // groups behind K: every activation there is zero, any scale will do
+        constexpr int RW = ROWS / kW4Warps;
+        for (int i = lane; i < want; i += 32) {
+            const int c = i < n ? i : n - 1;
+            uint32_t sv[RW], zv[RW];
 #pragma unroll
-        for (int r = 0; r < 2 * MT; r++) {
-            const uint16_t* sp = sbase + soff[r] + grp;
-            const uint8_t* zp = zbase + soff[r] + grp;
-            slot.z[r] = 0x08080808u;
-            if (G == 1) {
-                slot.s[r][0] = __ldg(sp);
-                if (zbase) slot.z[r] = __ldg(zp);
-            } else if (packed) {
-                if (G == 2) {
-                    slot.s[r][0] = __ldg(reinterpret_cast<const uint32_t*>(sp));
-                    if (zbase) slot.z[r] = __ldg(reinterpret_cast<const uint16_t*>(zp));
-                } else {
-                    const uint2 v = __ldg(reinterpret_cast<const uint2*>(sp));
-                    slot.s[r][0] = v.x;
-                    slot.s[r][G == 4 ? 1 : 0] = v.y;
-                    if (zbase) slot.z[r] = __ldg(reinterpret_cast<const uint32_t*>(zp));
-                }
-            } else {                                               // groups behind K: every activation there is zero, any scale will do
+            for (int q = 0; q < RW; q++) {
+                const int r = warp + q * kW4Warps;
+                const long long at = (base_row + (row0 + r < p.M ? r : p.M - 1 - row0)) * p.groups + g0 + c;
+                sv[q] = __ldg(p.scales + at);
+                zv[q] = p.zeros ? __ldg(p.zeros + at) & 15u : 8u;
+            }
 #pragma unroll
-                for (int q = 0; q < G; q++) {
-                    const int o = grp + q < p.groups ? q : p.groups - 1 - grp;
-                    const uint32_t v = __ldg(sp + o);
-                    if (q & 1) slot.s[r][q >> 1] |= v << 16;
-                    else slot.s[r][q >> 1] = v;
-                    if (zbase) slot.z[r] = (slot.z[r] & ~(255u << (8 * q))) | (uint32_t)__ldg(zp + o) << (8 * q);
-                }
+            for (int q = 0; q < RW; q++) {
+                const float zf = (float)zv[q] + (kHalf ? 0.f : W4Type<T>::kMagicValue);
+                s_sz[(warp + q * kW4Warps) * PITCH + i] = sv[q] | (uint32_t)W4Type<T>::from_float(zf) << 16;
             }
         }
     };
@@ -160,9 +164,7 @@ __global__ void __launch_bounds__(kW4Warps * 32, MT * NTL == 4 ? 1 : 2) w4_strea
 #pragma unroll
                 for (int e = 0; e < 4; e++) y[i][j][e] = 0.f;
 
-        // One block: products, then the slot is filled with the block after the next.
-        auto block = [&](W4Slot<MT, GW>& slot, int kb) {
-            uint4 b[4][NTL];
+        auto load_b = [&](uint4 (&b)[4][NTL], int kb) {
             if (kb < full_blocks) {
 #pragma unroll
                 for (int word = 0; word < 4; word++)
@@ -176,6 +178,11 @@ __global__ void __launch_bounds__(kW4Warps * 32, MT * NTL == 4 ? 1 : 2) w4_strea
                     for (int j = 0; j < NTL; j++) b[word][j] = load_x8(xrow[j] + k0, p.K - k0 - t * 8, p.x_vec != 0);
                 }
             }
+        };
+        auto block = [&](int at, const uint4 (&b)[4][NTL], const uint32_t* sz) {
+            uint4 slot[2 * MT];
+#pragma unroll
+            for (int r = 0; r < 2 * MT; r++) slot[r] = lds16(ring + at * (ROWS * kW4BlockBytes) + r * 512);
             float acc[MT][NTL][4], acc_hi[MT][NTL][4], gs[NTL][4];
 #pragma unroll
             for (int word = 0; word < 4; word++) {
@@ -192,7 +199,7 @@ __global__ void __launch_bounds__(kW4Warps * 32, MT * NTL == 4 ? 1 : 2) w4_strea
                 }
 #pragma unroll
                 for (int i = 0; i < MT; i++) {
-                    const uint4 u = slot.w[2 * i], v = slot.w[2 * i + 1];
+                    const uint4 u = slot[2 * i], v = slot[2 * i + 1];
                     const uint32_t wa = word == 0 ? u.x : (word == 1 ? u.y : (word == 2 ? u.z : u.w));
                     const uint32_t wb = word == 0 ? v.x : (word == 1 ? v.y : (word == 2 ? v.z : v.w));
                     if (kHalf) {
@@ -206,8 +213,8 @@ __global__ void __launch_bounds__(kW4Warps * 32, MT * NTL == 4 ? 1 : 2) w4_strea
                         uint32_t a[4], c[4];
 #pragma unroll
                         for (int q = 0; q < 4; q++) {
-                            a[q] = ((wa >> (4 * q)) & 0x000f000fu) | W4Type<T>::kMagic;
-                            c[q] = ((wb >> (4 * q)) & 0x000f000fu) | W4Type<T>::kMagic;
+                            a[q] = w4_field(wa >> (4 * q), 0x000f000fu, magic);
+                            c[q] = w4_field(wb >> (4 * q), 0x000f000fu, magic);
                         }
 #pragma unroll
                         for (int j = 0; j < NTL; j++) {
@@ -223,38 +230,46 @@ __global__ void __launch_bounds__(kW4Warps * 32, MT * NTL == 4 ? 1 : 2) w4_strea
                     mma16816<T>(gs[j], one, one, one, one, b[word][j].z, b[word][j].w);
                 }
                 if ((word + 1) % GW == 0) {                        // the end of a scale group
-                    const int q = word / GW;
 #pragma unroll
                     for (int i = 0; i < MT; i++) {
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            const float s = W4Type<T>::to_float((uint16_t)(slot.s[2 * i + h][q >> 1] >> (16 * (q & 1))));
-                            float z = (float)((slot.z[2 * i + h] >> (8 * q)) & 15u);
-                            if (!kHalf) z += W4Type<T>::kMagicValue;
+                            const float2 f = W4Type<T>::unpack2(sz[(i * 16 + h * 8) * PITCH + word / GW]);       // scale, zero point (+ magic)
 #pragma unroll
                             for (int j = 0; j < NTL; j++) {
 #pragma unroll
                                 for (int e = 0; e < 2; e++) {
                                     const int k = 2 * h + e;
                                     const float sum = kHalf ? fmaf(acc[i][j][k], 16777216.f, acc_hi[i][j][k] * 1048576.f) : acc[i][j][k] + acc_hi[i][j][k];
-                                    y[i][j][k] = fmaf(s, fmaf(-z, gs[j][e], sum), y[i][j][k]);
+                                    y[i][j][k] = fmaf(f.x, fmaf(-f.y, gs[j][e], sum), y[i][j][k]);
                                 }
                             }
                         }
                     }
                 }
             }
-            if (kb + 2 * kW4Warps < nblocks) fetch(slot, kb + 2 * kW4Warps);
         };
-        W4Slot<MT, GW> even, odd;
-        if (warp < nblocks) fetch(even, warp);
-        if (warp + kW4Warps < nblocks) fetch(odd, warp + kW4Warps);
+#pragma unroll
+        for (int d = 0; d < kW4Depth - 1; d++) fetch(d, warp + d * kW4Warps);
+        int at = 0;                                                // ring slot of the next block
+        for (int kc = 0; kc < nblocks; kc += kW4ChunkBlocks) {
+            if (kc || c0) __syncthreads();                         // the last pass over this memory is over
+            stage_scales(kc);
+            __syncthreads();
+            const int end = nblocks - kc < kW4ChunkBlocks ? nblocks : kc + kW4ChunkBlocks;
+            const uint32_t* sz = s_sz + g * PITCH + warp * G;
 #pragma unroll 1
-        for (int kb = warp; kb < nblocks; kb += 2 * kW4Warps) {
-            block(even, kb);
-            if (kb + kW4Warps < nblocks) block(odd, kb + kW4Warps);
+            for (int kb = kc + warp; kb < end; kb += kW4Warps, sz += kW4Warps * G) {
+                uint4 b[4][NTL];
+                load_b(b, kb);
+                fetch((at + kW4Depth - 1) % kW4Depth, kb + (kW4Depth - 1) * kW4Warps);      // into the slot read a step ago
+                copy_wait<kW4Depth - 1>();
+                block(at, b, sz);
+                at = (at + 1) % kW4Depth;
+            }
         }
         // the eight warps' sums, in a fixed order
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < MT; i++)
 #pragma unroll
@@ -262,8 +277,8 @@ __global__ void __launch_bounds__(kW4Warps * 32, MT * NTL == 4 ? 1 : 2) w4_strea
 #pragma unroll
                 for (int e = 0; e < 4; e++) red[warp][j * 8 + 2 * t + (e & 1)][i * 16 + g + 8 * (e >> 1)] = y[i][j][e];
         __syncthreads();
-        for (int o = threadIdx.x; o < NTL * 8 * MT * 16; o += kW4Warps * 32) {
-            const int n = o / (MT * 16), m = o % (MT * 16);
+        for (int o = threadIdx.x; o < NTL * 8 * ROWS; o += kW4Warps * 32) {
+            const int n = o / ROWS, m = o % ROWS;
             if (c0 + n < count && row0 + m < p.M) {
                 float v = 0.f;
 #pragma unroll
@@ -275,18 +290,32 @@ __global__ void __launch_bounds__(kW4Warps * 32, MT * NTL == 4 ? 1 : 2) w4_strea
                 static_cast<uint16_t*>(p.out)[(long long)(first + c0 + n) * p.out_ld + row0 + m] = W4Type<T>::from_float(v);
             }
         }
-        if (c0 + NTL * 8 < count) __syncthreads();
     }
 }
 
-template <typename T, int MT, int NTL>
-static int stream_groups(cudaStream_t stream, const W4Gemm& p, dim3 grid) {
-    cudaError_t e;
-    if (p.group == 32) e = launch_pdl(w4_stream_kernel<T, MT, NTL, 1>, grid, dim3(kW4Warps * 32), stream, p);
-    else if (p.group == 64) e = launch_pdl(w4_stream_kernel<T, MT, NTL, 2>, grid, dim3(kW4Warps * 32), stream, p);
-    else e = launch_pdl(w4_stream_kernel<T, MT, NTL, 4>, grid, dim3(kW4Warps * 32), stream, p);
+template <typename T, int MT, int NTL, int GW>
+static int stream_launch(cudaStream_t stream, const W4Gemm& p, dim3 grid) {
+    constexpr int ROWS = MT * 16;
+    constexpr int scale_bytes = ROWS * w4_pitch<GW>() * 4, sum_bytes = kW4Warps * NTL * 8 * (ROWS + 4) * 4;
+    constexpr int bytes = kW4Warps * kW4Depth * ROWS * kW4BlockBytes + (scale_bytes > sum_bytes ? scale_bytes : sum_bytes);
+    static_assert(bytes <= 227 * 1024, "shared memory of a CTA");
+    static bool configured[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 64 || !configured[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(w4_stream_kernel<T, MT, NTL, GW>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != cudaSuccess) return (int)e;
+        if (dev < 64) configured[dev] = true;
+    }
+    const cudaError_t e = launch_pdl_smem(w4_stream_kernel<T, MT, NTL, GW>, grid, dim3(kW4Warps * 32), (size_t)bytes, stream, p);
     count_launch();
     return (int)(e != cudaSuccess ? e : cudaGetLastError());
+}
+template <typename T, int MT, int NTL>
+static int stream_groups(cudaStream_t stream, const W4Gemm& p, dim3 grid) {
+    if (p.group == 32) return stream_launch<T, MT, NTL, 1>(stream, p, grid);
+    if (p.group == 64) return stream_launch<T, MT, NTL, 2>(stream, p, grid);
+    return stream_launch<T, MT, NTL, 4>(stream, p, grid);
 }
 
 template <typename T>

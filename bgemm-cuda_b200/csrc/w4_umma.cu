@@ -445,6 +445,7 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         constexpr int G = 4 / GW;                             // scale groups of a block
         bool ok = true;
+        const uint32_t magic = w4_opaque(W4Type<T>::kMagic);
         URing<C::W_STAGES> wring;                             // of the set's next block
         wring.step(set);
         uint32_t lap = 0;                                     // blocks of the set so far
@@ -500,7 +501,7 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
                         const uint32_t word[4] = {w == 0 ? c0.x : (w == 1 ? c0.y : (w == 2 ? c0.z : c0.w)), w == 0 ? c1.x : (w == 1 ? c1.y : (w == 2 ? c1.z : c1.w)),
                                                   w == 0 ? c2.x : (w == 1 ? c2.y : (w == 2 ? c2.z : c2.w)), w == 0 ? c3.x : (w == 1 ? c3.y : (w == 2 ? c3.z : c3.w))};
 #pragma unroll
-                        for (int e = 0; e < 16; e++) v[16 * q + e] = w4_pair<T>(word[e >> 2] >> (4 * (e & 3)), mz, s2);
+                        for (int e = 0; e < 16; e++) v[16 * q + e] = w4_pair<T>(word[e >> 2] >> (4 * (e & 3)), mz, s2, magic);
                     }
                     if (half == 0) {
                         if (lap) ok = mbar_wait(empty + 8 * set, (lap - 1) & 1, abort_flag, p.status, 58);
