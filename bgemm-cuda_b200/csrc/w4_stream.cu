@@ -10,7 +10,7 @@
 //         128 joins the zero point.
 //   The sums of x over a group, which the zero point needs, come from one more product with a matrix of ones.
 //
-// A CTA of eight warps owns 16 or 32 weight rows; its warps take the 128-column blocks of the rows in turn (adjacent warps
+// A CTA owns 16 or 32 weight rows; its warps take the 128-column blocks of the rows in turn (adjacent warps
 // read adjacent 64-byte pieces of a row) and their sums meet in shared memory, in a fixed order. Activations are read straight
 // from L1 / L2 in fragment order: there is nothing to stage, no limit on K, and a row index costs nothing.
 // Experts: blockIdx.y counts the experts that have rows; a CTA finds its own in the offsets.
@@ -22,7 +22,6 @@
 
 namespace bgemm {
 
-constexpr int kW4Warps = 8;
 
 // 16 bytes from global to shared memory, past L1, waited for by groups.
 __device__ __forceinline__ void copy16(uint32_t dst_smem, const void* src) {
@@ -37,19 +36,30 @@ __device__ __forceinline__ uint4 lds16(uint32_t addr) {
     return v;
 }
 
+// c = a b (first) or c += a b; `first` is a constant wherever this is inlined.
 template <typename T>
-__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, bool first);
 template <>
-__device__ __forceinline__ void mma16816<__half>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma16816<__half>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, bool first) {
+    if (first)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                     : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 template <>
-__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, bool first) {
+    if (first)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                     : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // Eight consecutive activations of one row; columns at or beyond `valid` read as zero.
@@ -64,19 +74,25 @@ __device__ __forceinline__ uint4 load_x8(const uint16_t* at, int valid, bool vec
 
 // Columns of one pass over the scales, which wait in shared memory as pairs (scale, zero point) of the 16-bit type.
 constexpr int kW4ChunkBlocks = 64;
-constexpr int kW4Depth = 4;                                                         // blocks of a warp on their way
+constexpr int kW4Depth = 3;                                                         // blocks of a warp on their way, the one at work included
 template <int GW>
-__host__ __device__ constexpr int w4_pitch() { return kW4ChunkBlocks * (4 / GW) + 1; }                  // odd: the eight rows of a warp's read meet eight banks
+__host__ __device__ constexpr int w4_pitch() { return kW4ChunkBlocks * (4 / GW) + 4; }                  // 4 mod 32, 16-byte rows: the eight rows of a read meet eight banks
 
-// MT: 16-row tiles of a CTA, NTL: 8-column tiles of activation rows per pass, GW: 32-column words per scale group (1, 2, 4).
-template <typename T, int MT, int NTL, int GW>
-__global__ void __launch_bounds__(kW4Warps * 32, MT * NTL == 4 ? 1 : 2) w4_stream_kernel(const W4Gemm p) {
+// Warps an SM is meant to hold: what the registers of H octets of rows and NTL column tiles leave room for.
+__host__ __device__ constexpr int w4_resident_warps(int H, int NTL) { return NTL == 2 ? (H > 2 ? 12 : 16) : (H > 4 ? 20 : 24); }
+
+// W: warps of a CTA (K is divided among them), H: its weight rows in octets (two make a 16-row product, an odd one a product
+// whose other half is zero), NTL: 8-column tiles of activation rows per pass, GW: 32-column words per scale group (1, 2, 4).
+template <typename T, int W, int H, int NTL, int GW>
+__global__ void __launch_bounds__(W * 32, w4_resident_warps(H, NTL) / W) w4_stream_kernel(const W4Gemm p) {
+    constexpr int MT = (H + 1) / 2;
     constexpr bool kHalf = W4Type<T>::kMagicValue == 1024.f;
-    constexpr int G = 4 / GW, PITCH = w4_pitch<GW>(), ROWS = MT * 16;
+    constexpr int G = 4 / GW, PITCH = w4_pitch<GW>(), ROWS = H * 8;
     // Per warp a ring of blocks that every lane fills and reads back itself (no barrier anywhere near it), then the scales
     // [ROWS][PITCH], where the warps' sums meet afterwards.
     extern __shared__ __align__(16) uint32_t smem[];
-    uint32_t* s_sz = smem + kW4Warps * kW4Depth * (ROWS * kW4BlockBytes / 4);
+    constexpr int STEP_BYTES = ROWS * kW4BlockBytes;
+    uint32_t* s_sz = smem + W * kW4Depth * (STEP_BYTES / 4);
     float(*red)[NTL * 8][ROWS + 4] = reinterpret_cast<float(*)[NTL * 8][ROWS + 4]>(s_sz);
     grid_dependency_wait();
     // the shuffle tells the compiler that the warp's number is uniform: block addresses are then computed by the uniform unit
@@ -108,32 +124,32 @@ __global__ void __launch_bounds__(kW4Warps * 32, MT * NTL == 4 ? 1 : 2) w4_strea
     const uint32_t magic = w4_opaque(W4Type<T>::kMagic);
     const long long base_row = (long long)expert * p.M + row0;
     const uint8_t* wbase = p.plane + base_row * p.row_bytes;
-    uint32_t woff[2 * MT];
+    uint32_t woff[H];
 #pragma unroll
-    for (int r = 0; r < 2 * MT; r++) {
+    for (int r = 0; r < H; r++) {
         const int m = row0 + r * 8 + g < p.M ? r * 8 + g : p.M - 1 - row0;     // rows behind the matrix repeat the last one and are not stored
         woff[r] = (uint32_t)m * (uint32_t)p.row_bytes + t * 16;
     }
-    const uint32_t ring = smem_u32(smem) + warp * (kW4Depth * ROWS * kW4BlockBytes) + lane * 16;
+    const uint32_t ring = smem_u32(smem) + warp * (kW4Depth * STEP_BYTES) + lane * 16;
     auto fetch = [&](int slot, int kb) {                           // a group is committed whether there is such a block or not
         if (kb < nblocks) {
             const uint8_t* at = wbase + (long long)kb * kW4BlockBytes;
 #pragma unroll
-            for (int r = 0; r < 2 * MT; r++) copy16(ring + slot * (ROWS * kW4BlockBytes) + r * 512, at + woff[r]);
+            for (int r = 0; r < H; r++) copy16(ring + slot * STEP_BYTES + r * 512, at + woff[r]);
         }
         copy_commit();
     };
     // scales and zero points of the blocks [kb0, kb0 + 64): coalesced along the rows
     auto stage_scales = [&](int kb0) {
         const int g0 = kb0 * G, n = p.groups - g0 < kW4ChunkBlocks * G ? p.groups - g0 : kW4ChunkBlocks * G;
-        const int want = (n + G - 1) / G * G;                      // groups behind K: every activation there is zero, any scale will do
-        constexpr int RW = ROWS / kW4Warps;
+        const int want = (n + G - 1) / G * G;      // groups behind K: every activation there is zero, any scale will do
+        constexpr int RW = (ROWS + W - 1) / W;
         for (int i = lane; i < want; i += 32) {
             const int c = i < n ? i : n - 1;
             uint32_t sv[RW], zv[RW];
 #pragma unroll
             for (int q = 0; q < RW; q++) {
-                const int r = warp + q * kW4Warps;
+                const int r = warp + q * W;
                 const long long at = (base_row + (row0 + r < p.M ? r : p.M - 1 - row0)) * p.groups + g0 + c;
                 sv[q] = __ldg(p.scales + at);
                 zv[q] = p.zeros ? __ldg(p.zeros + at) & 15u : 8u;
@@ -141,7 +157,7 @@ __global__ void __launch_bounds__(kW4Warps * 32, MT * NTL == 4 ? 1 : 2) w4_strea
 #pragma unroll
             for (int q = 0; q < RW; q++) {
                 const float zf = (float)zv[q] + (kHalf ? 0.f : W4Type<T>::kMagicValue);
-                s_sz[(warp + q * kW4Warps) * PITCH + i] = sv[q] | (uint32_t)W4Type<T>::from_float(zf) << 16;
+                if (warp + q * W < ROWS) s_sz[(warp + q * W) * PITCH + i] = sv[q] | (uint32_t)W4Type<T>::from_float(zf) << 16;
             }
         }
     };
@@ -179,68 +195,61 @@ __global__ void __launch_bounds__(kW4Warps * 32, MT * NTL == 4 ? 1 : 2) w4_strea
                 }
             }
         };
-        auto block = [&](int at, const uint4 (&b)[4][NTL], const uint32_t* sz) {
-            uint4 slot[2 * MT];
+        // The products of one block; sz: its first group of row g in the staged scales.
+        auto block = [&](uint32_t at, const uint4 (&b)[4][NTL], const uint32_t* sz) {
+            uint4 slot[H];
 #pragma unroll
-            for (int r = 0; r < 2 * MT; r++) slot[r] = lds16(ring + at * (ROWS * kW4BlockBytes) + r * 512);
+            for (int r = 0; r < H; r++) slot[r] = lds16(at + r * 512);
             float acc[MT][NTL][4], acc_hi[MT][NTL][4], gs[NTL][4];
 #pragma unroll
             for (int word = 0; word < 4; word++) {
-                if (word % GW == 0) {
-#pragma unroll
-                    for (int j = 0; j < NTL; j++) {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            gs[j][e] = 0.f;
-#pragma unroll
-                            for (int i = 0; i < MT; i++) acc[i][j][e] = acc_hi[i][j][e] = 0.f;
-                        }
-                    }
-                }
+                const bool first = word % GW == 0;
 #pragma unroll
                 for (int i = 0; i < MT; i++) {
-                    const uint4 u = slot[2 * i], v = slot[2 * i + 1];
+                    const bool both = 2 * i + 1 < H;               // a constant after unrolling
+                    const uint4 u = slot[2 * i], v = both ? slot[2 * i + 1 < H ? 2 * i + 1 : 0] : make_uint4(0, 0, 0, 0);
                     const uint32_t wa = word == 0 ? u.x : (word == 1 ? u.y : (word == 2 ? u.z : u.w));
                     const uint32_t wb = word == 0 ? v.x : (word == 1 ? v.y : (word == 2 ? v.z : v.w));
                     if (kHalf) {
                         const uint32_t ha = wa >> 8, hb = wb >> 8;
 #pragma unroll
                         for (int j = 0; j < NTL; j++) {
-                            mma16816<T>(acc[i][j], wa & 0x000f000fu, wb & 0x000f000fu, ha & 0x000f000fu, hb & 0x000f000fu, b[word][j].x, b[word][j].z);
-                            mma16816<T>(acc_hi[i][j], wa & 0x00f000f0u, wb & 0x00f000f0u, ha & 0x00f000f0u, hb & 0x00f000f0u, b[word][j].y, b[word][j].w);
+                            mma16816<T>(acc[i][j], wa & 0x000f000fu, wb & 0x000f000fu, ha & 0x000f000fu, hb & 0x000f000fu, b[word][j].x, b[word][j].z, first);
+                            mma16816<T>(acc_hi[i][j], wa & 0x00f000f0u, wb & 0x00f000f0u, ha & 0x00f000f0u, hb & 0x00f000f0u, b[word][j].y, b[word][j].w, first);
                         }
                     } else {
                         uint32_t a[4], c[4];
 #pragma unroll
                         for (int q = 0; q < 4; q++) {
                             a[q] = w4_field(wa >> (4 * q), 0x000f000fu, magic);
-                            c[q] = w4_field(wb >> (4 * q), 0x000f000fu, magic);
+                            c[q] = both ? w4_field(wb >> (4 * q), 0x000f000fu, magic) : 0u;
                         }
 #pragma unroll
                         for (int j = 0; j < NTL; j++) {
-                            mma16816<T>(acc[i][j], a[0], c[0], a[1], c[1], b[word][j].x, b[word][j].y);
-                            mma16816<T>(acc_hi[i][j], a[2], c[2], a[3], c[3], b[word][j].z, b[word][j].w);
+                            mma16816<T>(acc[i][j], a[0], c[0], a[1], c[1], b[word][j].x, b[word][j].y, first);
+                            mma16816<T>(acc[i][j], a[2], c[2], a[3], c[3], b[word][j].z, b[word][j].w, false);
                         }
                     }
                 }
                 constexpr uint32_t one = W4Type<T>::kOnes;
 #pragma unroll
                 for (int j = 0; j < NTL; j++) {
-                    mma16816<T>(gs[j], one, one, one, one, b[word][j].x, b[word][j].y);
-                    mma16816<T>(gs[j], one, one, one, one, b[word][j].z, b[word][j].w);
+                    mma16816<T>(gs[j], one, one, one, one, b[word][j].x, b[word][j].y, first);
+                    mma16816<T>(gs[j], one, one, one, one, b[word][j].z, b[word][j].w, false);
                 }
                 if ((word + 1) % GW == 0) {                        // the end of a scale group
 #pragma unroll
                     for (int i = 0; i < MT; i++) {
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
+                            if (2 * i + h >= H) continue;
                             const float2 f = W4Type<T>::unpack2(sz[(i * 16 + h * 8) * PITCH + word / GW]);       // scale, zero point (+ magic)
 #pragma unroll
                             for (int j = 0; j < NTL; j++) {
 #pragma unroll
                                 for (int e = 0; e < 2; e++) {
                                     const int k = 2 * h + e;
-                                    const float sum = kHalf ? fmaf(acc[i][j][k], 16777216.f, acc_hi[i][j][k] * 1048576.f) : acc[i][j][k] + acc_hi[i][j][k];
+                                    const float sum = kHalf ? fmaf(acc[i][j][k], 16777216.f, acc_hi[i][j][k] * 1048576.f) : acc[i][j][k];
                                     y[i][j][k] = fmaf(f.x, fmaf(-f.y, gs[j][e], sum), y[i][j][k]);
                                 }
                             }
@@ -250,7 +259,7 @@ __global__ void __launch_bounds__(kW4Warps * 32, MT * NTL == 4 ? 1 : 2) w4_strea
             }
         };
 #pragma unroll
-        for (int d = 0; d < kW4Depth - 1; d++) fetch(d, warp + d * kW4Warps);
+        for (int d = 0; d < kW4Depth - 1; d++) fetch(d, warp + d * W);
         int at = 0;                                                // ring slot of the next block
         for (int kc = 0; kc < nblocks; kc += kW4ChunkBlocks) {
             if (kc || c0) __syncthreads();                         // the last pass over this memory is over
@@ -259,30 +268,31 @@ __global__ void __launch_bounds__(kW4Warps * 32, MT * NTL == 4 ? 1 : 2) w4_strea
             const int end = nblocks - kc < kW4ChunkBlocks ? nblocks : kc + kW4ChunkBlocks;
             const uint32_t* sz = s_sz + g * PITCH + warp * G;
 #pragma unroll 1
-            for (int kb = kc + warp; kb < end; kb += kW4Warps, sz += kW4Warps * G) {
+            for (int kb = kc + warp; kb < end; kb += W, sz += W * G) {
                 uint4 b[4][NTL];
                 load_b(b, kb);
-                fetch((at + kW4Depth - 1) % kW4Depth, kb + (kW4Depth - 1) * kW4Warps);      // into the slot read a step ago
+                fetch(at + kW4Depth - 1 >= kW4Depth ? at - 1 : at + kW4Depth - 1, kb + (kW4Depth - 1) * W);      // into the slot read a step ago
                 copy_wait<kW4Depth - 1>();
-                block(at, b, sz);
-                at = (at + 1) % kW4Depth;
+                block(ring + at * STEP_BYTES, b, sz);
+                at = at + 1 == kW4Depth ? 0 : at + 1;
             }
         }
-        // the eight warps' sums, in a fixed order
+        // the warps' sums, in a fixed order
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < MT; i++)
 #pragma unroll
             for (int j = 0; j < NTL; j++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) red[warp][j * 8 + 2 * t + (e & 1)][i * 16 + g + 8 * (e >> 1)] = y[i][j][e];
+                for (int e = 0; e < 4; e++)
+                    if (2 * i + (e >> 1) < H) red[warp][j * 8 + 2 * t + (e & 1)][i * 16 + g + 8 * (e >> 1)] = y[i][j][e];
         __syncthreads();
-        for (int o = threadIdx.x; o < NTL * 8 * ROWS; o += kW4Warps * 32) {
+        for (int o = threadIdx.x; o < NTL * 8 * ROWS; o += W * 32) {
             const int n = o / ROWS, m = o % ROWS;
             if (c0 + n < count && row0 + m < p.M) {
                 float v = 0.f;
 #pragma unroll
-                for (int q = 0; q < kW4Warps; q++) v += red[q][n][m];
+                for (int q = 0; q < W; q++) v += red[q][n][m];
                 if (p.rows) {
                     const int src = p.rows[first + c0 + n];
                     if (src < 0 || src >= p.x_rows) v = 0.f;
@@ -293,39 +303,52 @@ __global__ void __launch_bounds__(kW4Warps * 32, MT * NTL == 4 ? 1 : 2) w4_strea
     }
 }
 
-template <typename T, int MT, int NTL, int GW>
+template <typename T, int W, int H, int NTL, int GW>
 static int stream_launch(cudaStream_t stream, const W4Gemm& p, dim3 grid) {
-    constexpr int ROWS = MT * 16;
-    constexpr int scale_bytes = ROWS * w4_pitch<GW>() * 4, sum_bytes = kW4Warps * NTL * 8 * (ROWS + 4) * 4;
-    constexpr int bytes = kW4Warps * kW4Depth * ROWS * kW4BlockBytes + (scale_bytes > sum_bytes ? scale_bytes : sum_bytes);
+    constexpr int ROWS = H * 8;
+    constexpr int scale_bytes = ROWS * w4_pitch<GW>() * 4, sum_bytes = W * NTL * 8 * (ROWS + 4) * 4;
+    constexpr int bytes = W * kW4Depth * ROWS * kW4BlockBytes + (scale_bytes > sum_bytes ? scale_bytes : sum_bytes);
     static_assert(bytes <= 227 * 1024, "shared memory of a CTA");
     static bool configured[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 64 || !configured[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(w4_stream_kernel<T, MT, NTL, GW>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        const cudaError_t e = cudaFuncSetAttribute(w4_stream_kernel<T, W, H, NTL, GW>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
         if (e != cudaSuccess) return (int)e;
         if (dev < 64) configured[dev] = true;
     }
-    const cudaError_t e = launch_pdl_smem(w4_stream_kernel<T, MT, NTL, GW>, grid, dim3(kW4Warps * 32), (size_t)bytes, stream, p);
+    const cudaError_t e = launch_pdl_smem(w4_stream_kernel<T, W, H, NTL, GW>, grid, dim3(W * 32), (size_t)bytes, stream, p);
     count_launch();
     return (int)(e != cudaSuccess ? e : cudaGetLastError());
 }
-template <typename T, int MT, int NTL>
-static int stream_groups(cudaStream_t stream, const W4Gemm& p, dim3 grid) {
-    if (p.group == 32) return stream_launch<T, MT, NTL, 1>(stream, p, grid);
-    if (p.group == 64) return stream_launch<T, MT, NTL, 2>(stream, p, grid);
-    return stream_launch<T, MT, NTL, 4>(stream, p, grid);
+template <typename T, int W, int H, int NTL>
+static int stream_groups(cudaStream_t stream, const W4Gemm& p, long long experts) {
+    const dim3 grid((unsigned)((p.M + H * 8 - 1) / (H * 8)), (unsigned)experts);
+    if (p.group == 32) return stream_launch<T, W, H, NTL, 1>(stream, p, grid);
+    if (p.group == 64) return stream_launch<T, W, H, NTL, 2>(stream, p, grid);
+    return stream_launch<T, W, H, NTL, 4>(stream, p, grid);
 }
 
+// Warps and rows of a CTA. The launch lasts as long as the SM with the most rows (a tile more than an SM's share is a seventh
+// more time at six tiles an SM: 28672 x 8192 on one row took 32.3 us in tiles of 32 rows, 896 of them, and 28.4 in tiles of
+// 40, 717), so of 32 and 40 rows the one with the lower maximum is taken. Few tiles: smaller ones, and more warps to share
+// their K. Measured against the others (us, one row): 1024 x 4096 12 warps x 16 rows 3.33, 8 x 16 3.44, 4 x 32 5.19; 4096 x
+// 4096 8 x 16 5.52, 8 x 32 5.98, 4 x 32 6.90; 8192 x 8192 8 x 32 12.4, 8 x 16 13.6, 4 x 32 13.1; 11008 x 4096 8 x 40 8.98,
+// 4 x 40 9.24, 8 x 16 10.3; 14336 x 4096 4 x 40 11.0, 4 x 32 11.2, 8 x 40 13.1.
 template <typename T>
 static int stream_variant(cudaStream_t stream, const W4Gemm& p) {
-    const long long experts = p.offsets ? (p.slots < p.E ? p.slots : p.E) : 1;
-    const bool wide = (p.M + 31) / 32 * experts >= 2 * sm_count();
-    const bool two = p.slots > 8 * experts;
-    const dim3 grid((unsigned)((p.M + (wide ? 31 : 15)) / (wide ? 32 : 16)), (unsigned)experts);
-    if (wide) return two ? stream_groups<T, 2, 2>(stream, p, grid) : stream_groups<T, 2, 1>(stream, p, grid);
-    return two ? stream_groups<T, 1, 2>(stream, p, grid) : stream_groups<T, 1, 1>(stream, p, grid);
+    const long long experts = p.offsets ? (p.slots < p.E ? p.slots : p.E) : 1, sms = sm_count();
+    const auto tiles = [&](int rows) { return (p.M + rows - 1) / rows * experts; };
+    const auto most_rows = [&](int rows) { return (tiles(rows) + sms - 1) / sms * rows; };
+    if (p.slots > 8 * experts) {          // two column tiles a pass (4096 x 4096 on 16 rows: 8 x 16 7.7, 4 x 32 8.7; 28672 x 8192: 63, 53)
+        if (tiles(16) <= 2 * sms) return stream_groups<T, 8, 2, 2>(stream, p, experts);
+        return stream_groups<T, 4, 4, 2>(stream, p, experts);
+    }
+    if (tiles(16) <= sms) return stream_groups<T, 12, 2, 1>(stream, p, experts);
+    if (tiles(16) <= 2 * sms) return stream_groups<T, 8, 2, 1>(stream, p, experts);
+    const bool forty = most_rows(40) < most_rows(32), shared = 2 * tiles(32) <= 5 * sms;
+    if (shared) return forty ? stream_groups<T, 8, 5, 1>(stream, p, experts) : stream_groups<T, 8, 4, 1>(stream, p, experts);
+    return forty ? stream_groups<T, 4, 5, 1>(stream, p, experts) : stream_groups<T, 4, 4, 1>(stream, p, experts);
 }
 
 int launch_w4_stream(cudaStream_t stream, const W4Gemm& p, int dtype) {

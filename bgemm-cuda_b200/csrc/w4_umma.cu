@@ -49,13 +49,18 @@ struct UCfg {
     static constexpr int STAGES = 4, A_STAGE_COLS = 64, A_COL0 = NT;
     static constexpr int B_SUB_BYTES = 128 * 128;           // 64 columns of this CTA's half of the activation rows
     static constexpr int B_STAGE_BYTES = 2 * B_SUB_BYTES;
-    static constexpr int W_STAGES = 6, W_STAGE_BYTES = 128 * kW4BlockBytes;
+    static constexpr int W_STAGES = 8, W_STAGE_BYTES = 128 * kW4BlockBytes;
     static constexpr int PITCH = 272;                       // bytes of a staged result column: 128 x 2 + 16
-    static constexpr int STAGING_BYTES = 128 * PITCH;       // 64 columns per epilogue half
+    static constexpr int STAGED = 32;                       // result columns staged at a time, per epilogue half
+    static constexpr int STAGING_BYTES = 2 * STAGED * PITCH;
     // w_full/w_empty, full/empty, d_full[2], d_empty[2], drained
     static constexpr int NBARS = 2 * W_STAGES + 2 * STAGES + 5;
     static constexpr int MISC_BYTES = 512 + 2 * 4 * (kUMaxExperts + 8);
     static constexpr int SMEM_BYTES = STAGES * B_STAGE_BYTES + W_STAGES * W_STAGE_BYTES + STAGING_BYTES + MISC_BYTES + 1024;
+    // A stage and its barriers always meet the same set (and the same producer warp): a set that waits for a phase by its
+    // parity has then seen the phase before it complete. With six code stages and four sets it had not, and a code copy that was
+    // overtaken by a later one let a set read a stage that was still being filled.
+    static_assert(W_STAGES % kUSets == 0 && STAGES % 2 == 0, "stage -> unpack set / producer must stay fixed");
     static_assert(STAGES == kUSets, "an operand stage always meets the same unpack set");
     static_assert(NBARS * 8 <= 320, "barrier area");
     static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
@@ -524,7 +529,7 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
         const int hw = (warp - kUWarpEpi) >> 2;
         const int et = (warp & 3) * 32 + lane;                // weight row == tensor-memory lane; also the thread's number in its group
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-        uint8_t* stage = sOut + hw * 64 * C::PITCH;
+        uint8_t* stage = sOut + hw * C::STAGED * C::PITCH;
         const bool vec = p.g.out_ld % 8 == 0 && (reinterpret_cast<uintptr_t>(p.g.out) & 15) == 0;
         UHalves h;
         for (int t = cid; t < total; t += ncl) {
@@ -536,8 +541,8 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
             const int ncols = u.n >> 1, col0 = hw * ncols;    // a multiple of 16
             const uint32_t acc = tmem + h.lead * 128 + lane_base + col0;
             const int m0 = u.m0 + (int)rank * 128;
-            for (int c0 = 0; c0 < ncols; c0 += 64) {
-                const int nc = ncols - c0 < 64 ? ncols - c0 : 64;
+            for (int c0 = 0; c0 < ncols; c0 += C::STAGED) {
+                const int nc = ncols - c0 < C::STAGED ? ncols - c0 : C::STAGED;
                 if (c0) named_bar_sync(1 + hw, 128);          // the staging columns have been stored
                 for (int c = 0; c < nc; c += 16) {
                     uint32_t v[16];
@@ -557,7 +562,7 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
                             *reinterpret_cast<uint16_t*>(stage + (c + q) * C::PITCH + et * 2) = W4Type<T>::from_float(__uint_as_float(v[q]));
                     }
                 }
-                if (c0 + 64 >= ncols) {                       // everything is out of the accumulator
+                if (c0 + C::STAGED >= ncols) {                       // everything is out of the accumulator
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
