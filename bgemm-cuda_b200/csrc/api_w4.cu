@@ -1,5 +1,4 @@
 // extern "C" surface of the 4-bit weight products and the expert routing (include/bgemm_b200.h): argument checks and launches.
-#include <cstdlib>
 #include "internal.h"
 #include "w4.cuh"
 
@@ -47,13 +46,21 @@ W4Gemm problem(const void* plane, int E, int64_t M, int64_t K, int group, const 
     return p;
 }
 
-// Up to 16 rows per matrix the product is bound by the weights' bytes and the register-fed kernel takes it; beyond, the
-// tensor cores. Rows of x off 16-byte boundaries cannot be loaded by TMA and stay on the former, whatever their number.
+// Which kernel. The streaming kernel passes over a matrix once for every eight rows that meet it and wants ~5 us a
+// megabyte and pass less than the tensor-core kernel to begin with, which takes any number of rows in one pass but ~9 us to
+// fill and drain. Measured (us, streaming / tensor cores): 4096 x 4096 on 16 rows 8 / 15, on 24 10 / 15, on 32 14 / 15;
+// 11008 x 4096 on 16 rows 16 / 18, on 24 22 / 18; 28672 x 8192 on 8 rows 31 / 51, on 16 58 / 51; 64 experts of 2048 x 4096 on 8 rows
+// each 72 / 98, on 12 129 / 99; 8 of them on 93 rows 24 / 20. Rows of x off 16-byte boundaries cannot be loaded by TMA and stay on the former.
 bool on_tensor_cores(const W4Gemm& p) {
-    const long long experts = p.offsets ? (p.slots < p.E ? p.slots : p.E) : 1;
-    static const int f = std::getenv("W4PATH") ? std::atoi(std::getenv("W4PATH")) : -1;
-    if (f >= 0) return p.x_vec && f;
-    return p.x_vec && p.slots > 16 && p.slots > 8 * experts;
+    if (!p.x_vec) return false;
+    const double matrix = (double)p.M * (double)p.K / 2;
+    if (!p.offsets) {
+        const long long passes = (p.slots + 7) / 8;
+        return passes > 1 && passes * matrix > 45e6;
+    }
+    // the counts are on the device: on average an expert's last pass is not full
+    const double experts = (double)(p.slots < p.E ? p.slots : p.E), rows = (double)p.slots / experts;
+    return rows > 6 && experts * (rows / 8 + 0.4) * matrix > 45e6;
 }
 
 int run(cudaStream_t stream, const W4Gemm& p, int dtype, void* workspace, size_t workspace_bytes) {

@@ -30,9 +30,9 @@ __device__ __forceinline__ void copy16(uint32_t dst_smem, const void* src) {
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ uint4 lds16(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+__device__ __forceinline__ uint2 lds8(uint32_t addr) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
     return v;
 }
 
@@ -78,50 +78,74 @@ constexpr int kW4Depth = 3;                                                     
 template <int GW>
 __host__ __device__ constexpr int w4_pitch() { return kW4ChunkBlocks * (4 / GW) + 4; }                  // 4 mod 32, 16-byte rows: the eight rows of a read meet eight banks
 
-// Warps an SM is meant to hold: what the registers of H octets of rows and NTL column tiles leave room for.
-__host__ __device__ constexpr int w4_resident_warps(int H, int NTL) { return NTL == 2 ? (H > 2 ? 12 : 16) : (H > 4 ? 20 : 24); }
+// Warps an SM is meant to hold. Five octets of fp16 rows spill at what 24 leave each (28672 x 8192 on 8 rows in groups of 64:
+// 47 us, 40 with 20 warps); bf16 does not (31.1, 32.3 with 20).
+template <typename T>
+__host__ __device__ constexpr int w4_resident_warps(int H) { return H > 4 && W4Type<T>::kMagicValue == 1024.f ? 20 : 24; }
 
 // W: warps of a CTA (K is divided among them), H: its weight rows in octets (two make a 16-row product, an odd one a product
-// whose other half is zero), NTL: 8-column tiles of activation rows per pass, GW: 32-column words per scale group (1, 2, 4).
-template <typename T, int W, int H, int NTL, int GW>
-__global__ void __launch_bounds__(W * 32, w4_resident_warps(H, NTL) / W) w4_stream_kernel(const W4Gemm p) {
-    constexpr int MT = (H + 1) / 2;
+// whose other half is zero), GW: 32-column words per scale group (1, 2, 4).
+template <typename T, int W, int H, int GW>
+__global__ void __launch_bounds__(W * 32, w4_resident_warps<T>(H) / W) w4_stream_kernel(const W4Gemm p) {
     constexpr bool kHalf = W4Type<T>::kMagicValue == 1024.f;
-    constexpr int G = 4 / GW, PITCH = w4_pitch<GW>(), ROWS = H * 8;
+    constexpr int MT = (H + 1) / 2, G = 4 / GW, PITCH = w4_pitch<GW>(), ROWS = H * 8, STEP_BYTES = ROWS * kW4BlockBytes;
     // Per warp a ring of blocks that every lane fills and reads back itself (no barrier anywhere near it), then the scales
     // [ROWS][PITCH], where the warps' sums meet afterwards.
     extern __shared__ __align__(16) uint32_t smem[];
-    constexpr int STEP_BYTES = ROWS * kW4BlockBytes;
     uint32_t* s_sz = smem + W * kW4Depth * (STEP_BYTES / 4);
-    float(*red)[NTL * 8][ROWS + 4] = reinterpret_cast<float(*)[NTL * 8][ROWS + 4]>(s_sz);
+    float(*red)[8][ROWS + 4] = reinterpret_cast<float(*)[8][ROWS + 4]>(s_sz);
     grid_dependency_wait();
     // the shuffle tells the compiler that the warp's number is uniform: block addresses are then computed by the uniform unit
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), g = lane >> 2, t = lane & 3;
 
-    int expert = 0, first, count;
-    if (p.offsets) {                                               // the blockIdx.y-th expert that has rows
-        int want = blockIdx.y;
-        bool found = false;
-        for (int base = 0; base < p.E && !found; base += 32) {
+    // This CTA's expert and its eight rows: the blockIdx.y-th group of eight, experts in order.
+    int expert = 0, first = 0, count;
+    if (p.offsets) {
+        // lane l looks at experts [l q, (l + 1) q): all loads are on their way at once, one prefix sum over the warp
+        const int q = (p.E + 31) / 32;
+        int mine = 0;
+        for (int i = 0; i < q; i++) {
             int f = 0, c = 0;
-            if (base + lane < p.E) w4_expert_range(p, base + lane, f, c);
-            const uint32_t has = __ballot_sync(0xffffffffu, c > 0);
-            const int n = __popc(has);
-            if (want < n) {
-                expert = base + (int)__fns(has, 0, want + 1);
-                found = true;
-            }
-            want -= n;
+            if (lane * q + i < p.E) w4_expert_range(p, lane * q + i, f, c);
+            mine += (c + 7) / 8;
         }
-        if (!found) return;
+        int before = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, before, d);
+            if (lane >= d) before += up;
+        }
+        before -= mine;
+        const int want = blockIdx.y;
+        const uint32_t has = __ballot_sync(0xffffffffu, want >= before && want < before + mine);
+        if (!has) return;
+        int found = 0, skip = 0;
+        if (want >= before && want < before + mine) {
+            int at = want - before;
+            for (int i = 0; i < q; i++) {
+                int f = 0, c = 0;
+                if (lane * q + i < p.E) w4_expert_range(p, lane * q + i, f, c);
+                const int n = (c + 7) / 8;
+                if (at >= 0 && at < n) {
+                    found = lane * q + i;
+                    skip = at * 8;
+                }
+                at -= n;
+            }
+        }
+        const int owner = __ffs(has) - 1;
+        expert = __shfl_sync(0xffffffffu, found, owner);
+        skip = __shfl_sync(0xffffffffu, skip, owner);
+        w4_expert_range(p, expert, first, count);
+        first += skip;
+        count -= skip;
+    } else {
+        first = blockIdx.y * 8;
+        count = (int)p.slots - first;
     }
-    w4_expert_range(p, expert, first, count);
-    expert = __shfl_sync(0xffffffffu, expert, 0);
 
     const int row0 = blockIdx.x * ROWS;
     const int nblocks = (p.K + kW4Block - 1) / kW4Block;
-    const int full_blocks = p.x_vec ? p.K / kW4Block : 0;          // blocks whose activations are whole 16-byte pieces
-    const uint32_t magic = w4_opaque(W4Type<T>::kMagic);
     const long long base_row = (long long)expert * p.M + row0;
     const uint8_t* wbase = p.plane + base_row * p.row_bytes;
     uint32_t woff[H];
@@ -139,10 +163,13 @@ __global__ void __launch_bounds__(W * 32, w4_resident_warps(H, NTL) / W) w4_stre
         }
         copy_commit();
     };
+#pragma unroll
+    for (int d = 0; d < kW4Depth - 1; d++) fetch(d, warp + d * W);
+
     // scales and zero points of the blocks [kb0, kb0 + 64): coalesced along the rows
     auto stage_scales = [&](int kb0) {
         const int g0 = kb0 * G, n = p.groups - g0 < kW4ChunkBlocks * G ? p.groups - g0 : kW4ChunkBlocks * G;
-        const int want = (n + G - 1) / G * G;      // groups behind K: every activation there is zero, any scale will do
+        const int want = (n + G - 1) / G * G;                      // groups behind K: every activation there is zero, any scale will do
         constexpr int RW = (ROWS + W - 1) / W;
         for (int i = lane; i < want; i += 32) {
             const int c = i < n ? i : n - 1;
@@ -162,171 +189,161 @@ __global__ void __launch_bounds__(W * 32, w4_resident_warps(H, NTL) / W) w4_stre
         }
     };
 
-    for (int c0 = 0; c0 < count; c0 += NTL * 8) {
-        const uint16_t* xrow[NTL];
+    // columns behind the expert's rows and rows outside x repeat a row that exists; the former are not stored, the latter
+    // stored as zeros (a column of the product sees nothing of the others)
+    const uint16_t* xrow;
+    {
+        const int n = g < count ? g : count - 1;
+        const long long src = p.rows ? (long long)p.rows[first + n] : (long long)first + n;
+        xrow = static_cast<const uint16_t*>(p.x) + (src >= 0 && src < p.x_rows ? src : 0) * p.x_ld + t * 8;
+    }
+    const int full_blocks = p.x_vec ? p.K / kW4Block : 0;          // blocks whose activations are whole 16-byte pieces
+    const uint32_t magic = w4_opaque(W4Type<T>::kMagic);
+    constexpr uint32_t one = W4Type<T>::kOnes;
+    float y[MT][4];
 #pragma unroll
-        for (int j = 0; j < NTL; j++) {
-            // columns behind the expert's rows and rows outside x repeat a row that exists; the former are not stored, the
-            // latter stored as zeros (a column of the product sees nothing of the others)
-            const int n = c0 + j * 8 + g < count ? c0 + j * 8 + g : count - 1;
-            const long long src = p.rows ? (long long)p.rows[first + n] : (long long)first + n;
-            xrow[j] = static_cast<const uint16_t*>(p.x) + (src >= 0 && src < p.x_rows ? src : 0) * p.x_ld + t * 8;
-        }
-        float y[MT][NTL][4];
+    for (int i = 0; i < MT; i++)
 #pragma unroll
-        for (int i = 0; i < MT; i++)
-#pragma unroll
-            for (int j = 0; j < NTL; j++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) y[i][j][e] = 0.f;
+        for (int e = 0; e < 4; e++) y[i][e] = 0.f;
 
-        auto load_b = [&](uint4 (&b)[4][NTL], int kb) {
-            if (kb < full_blocks) {
+    auto load_b = [&](uint4 (&b)[4], int kb) {
+        if (kb < full_blocks) {
 #pragma unroll
-                for (int word = 0; word < 4; word++)
-#pragma unroll
-                    for (int j = 0; j < NTL; j++) b[word][j] = __ldg(reinterpret_cast<const uint4*>(xrow[j] + kb * kW4Block + word * 32));
-            } else {
-#pragma unroll
-                for (int word = 0; word < 4; word++) {
-                    const int k0 = kb * kW4Block + word * 32;
-#pragma unroll
-                    for (int j = 0; j < NTL; j++) b[word][j] = load_x8(xrow[j] + k0, p.K - k0 - t * 8, p.x_vec != 0);
-                }
-            }
-        };
-        // The products of one block; sz: its first group of row g in the staged scales.
-        auto block = [&](uint32_t at, const uint4 (&b)[4][NTL], const uint32_t* sz) {
-            uint4 slot[H];
-#pragma unroll
-            for (int r = 0; r < H; r++) slot[r] = lds16(at + r * 512);
-            float acc[MT][NTL][4], acc_hi[MT][NTL][4], gs[NTL][4];
+            for (int word = 0; word < 4; word++) b[word] = __ldg(reinterpret_cast<const uint4*>(xrow + kb * kW4Block + word * 32));
+        } else {
 #pragma unroll
             for (int word = 0; word < 4; word++) {
-                const bool first = word % GW == 0;
-#pragma unroll
-                for (int i = 0; i < MT; i++) {
-                    const bool both = 2 * i + 1 < H;               // a constant after unrolling
-                    const uint4 u = slot[2 * i], v = both ? slot[2 * i + 1 < H ? 2 * i + 1 : 0] : make_uint4(0, 0, 0, 0);
-                    const uint32_t wa = word == 0 ? u.x : (word == 1 ? u.y : (word == 2 ? u.z : u.w));
-                    const uint32_t wb = word == 0 ? v.x : (word == 1 ? v.y : (word == 2 ? v.z : v.w));
-                    if (kHalf) {
-                        const uint32_t ha = wa >> 8, hb = wb >> 8;
-#pragma unroll
-                        for (int j = 0; j < NTL; j++) {
-                            mma16816<T>(acc[i][j], wa & 0x000f000fu, wb & 0x000f000fu, ha & 0x000f000fu, hb & 0x000f000fu, b[word][j].x, b[word][j].z, first);
-                            mma16816<T>(acc_hi[i][j], wa & 0x00f000f0u, wb & 0x00f000f0u, ha & 0x00f000f0u, hb & 0x00f000f0u, b[word][j].y, b[word][j].w, first);
-                        }
-                    } else {
-                        uint32_t a[4], c[4];
-#pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            a[q] = w4_field(wa >> (4 * q), 0x000f000fu, magic);
-                            c[q] = both ? w4_field(wb >> (4 * q), 0x000f000fu, magic) : 0u;
-                        }
-#pragma unroll
-                        for (int j = 0; j < NTL; j++) {
-                            mma16816<T>(acc[i][j], a[0], c[0], a[1], c[1], b[word][j].x, b[word][j].y, first);
-                            mma16816<T>(acc[i][j], a[2], c[2], a[3], c[3], b[word][j].z, b[word][j].w, false);
-                        }
-                    }
-                }
-                constexpr uint32_t one = W4Type<T>::kOnes;
-#pragma unroll
-                for (int j = 0; j < NTL; j++) {
-                    mma16816<T>(gs[j], one, one, one, one, b[word][j].x, b[word][j].y, first);
-                    mma16816<T>(gs[j], one, one, one, one, b[word][j].z, b[word][j].w, false);
-                }
-                if ((word + 1) % GW == 0) {                        // the end of a scale group
-#pragma unroll
-                    for (int i = 0; i < MT; i++) {
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            if (2 * i + h >= H) continue;
-                            const float2 f = W4Type<T>::unpack2(sz[(i * 16 + h * 8) * PITCH + word / GW]);       // scale, zero point (+ magic)
-#pragma unroll
-                            for (int j = 0; j < NTL; j++) {
-#pragma unroll
-                                for (int e = 0; e < 2; e++) {
-                                    const int k = 2 * h + e;
-                                    const float sum = kHalf ? fmaf(acc[i][j][k], 16777216.f, acc_hi[i][j][k] * 1048576.f) : acc[i][j][k];
-                                    y[i][j][k] = fmaf(f.x, fmaf(-f.y, gs[j][e], sum), y[i][j][k]);
-                                }
-                            }
-                        }
-                    }
-                }
-            }
-        };
-#pragma unroll
-        for (int d = 0; d < kW4Depth - 1; d++) fetch(d, warp + d * W);
-        int at = 0;                                                // ring slot of the next block
-        for (int kc = 0; kc < nblocks; kc += kW4ChunkBlocks) {
-            if (kc || c0) __syncthreads();                         // the last pass over this memory is over
-            stage_scales(kc);
-            __syncthreads();
-            const int end = nblocks - kc < kW4ChunkBlocks ? nblocks : kc + kW4ChunkBlocks;
-            const uint32_t* sz = s_sz + g * PITCH + warp * G;
-#pragma unroll 1
-            for (int kb = kc + warp; kb < end; kb += W, sz += W * G) {
-                uint4 b[4][NTL];
-                load_b(b, kb);
-                fetch(at + kW4Depth - 1 >= kW4Depth ? at - 1 : at + kW4Depth - 1, kb + (kW4Depth - 1) * W);      // into the slot read a step ago
-                copy_wait<kW4Depth - 1>();
-                block(ring + at * STEP_BYTES, b, sz);
-                at = at + 1 == kW4Depth ? 0 : at + 1;
+                const int k0 = kb * kW4Block + word * 32;
+                b[word] = load_x8(xrow + k0, p.K - k0 - t * 8, p.x_vec != 0);
             }
         }
-        // the warps' sums, in a fixed order
-        __syncthreads();
+    };
+    // The products of one block; sz: its first group of row g in the staged scales.
+    auto block = [&](uint32_t at, const uint4 (&b)[4], const uint32_t* sz) {
+        uint2 slot[H];                                             // two words of each row at a time: registers are what limits the warps
+        float acc[MT][4], acc_hi[MT][4], gs[4];
 #pragma unroll
-        for (int i = 0; i < MT; i++)
+        for (int word = 0; word < 4; word++) {
+            const bool start = word % GW == 0;
+            if (word % 2 == 0) {
 #pragma unroll
-            for (int j = 0; j < NTL; j++)
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (2 * i + (e >> 1) < H) red[warp][j * 8 + 2 * t + (e & 1)][i * 16 + g + 8 * (e >> 1)] = y[i][j][e];
-        __syncthreads();
-        for (int o = threadIdx.x; o < NTL * 8 * ROWS; o += W * 32) {
-            const int n = o / ROWS, m = o % ROWS;
-            if (c0 + n < count && row0 + m < p.M) {
-                float v = 0.f;
-#pragma unroll
-                for (int q = 0; q < W; q++) v += red[q][n][m];
-                if (p.rows) {
-                    const int src = p.rows[first + c0 + n];
-                    if (src < 0 || src >= p.x_rows) v = 0.f;
-                }
-                static_cast<uint16_t*>(p.out)[(long long)(first + c0 + n) * p.out_ld + row0 + m] = W4Type<T>::from_float(v);
+                for (int r = 0; r < H; r++) slot[r] = lds8(at + r * 512 + word * 4);
             }
+#pragma unroll
+            for (int i = 0; i < MT; i++) {
+                const bool both = 2 * i + 1 < H;                   // a constant after unrolling
+                const uint2 u = slot[2 * i], v = both ? slot[both ? 2 * i + 1 : 0] : make_uint2(0, 0);
+                const uint32_t wa = word % 2 ? u.y : u.x, wb = word % 2 ? v.y : v.x;
+                if (kHalf) {
+                    const uint32_t ha = wa >> 8, hb = wb >> 8;
+                    mma16816<T>(acc[i], wa & 0x000f000fu, wb & 0x000f000fu, ha & 0x000f000fu, hb & 0x000f000fu, b[word].x, b[word].z, start);
+                    mma16816<T>(acc_hi[i], wa & 0x00f000f0u, wb & 0x00f000f0u, ha & 0x00f000f0u, hb & 0x00f000f0u, b[word].y, b[word].w, start);
+                } else {
+                    uint32_t a[4], c[4];
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        a[q] = w4_field(wa >> (4 * q), 0x000f000fu, magic);
+                        c[q] = both ? w4_field(wb >> (4 * q), 0x000f000fu, magic) : 0u;
+                    }
+                    mma16816<T>(acc[i], a[0], c[0], a[1], c[1], b[word].x, b[word].y, start);
+                    mma16816<T>(acc[i], a[2], c[2], a[3], c[3], b[word].z, b[word].w, false);
+                }
+            }
+            mma16816<T>(gs, one, one, one, one, b[word].x, b[word].y, start);
+            mma16816<T>(gs, one, one, one, one, b[word].z, b[word].w, false);
+            if ((word + 1) % GW == 0) {                            // the end of a scale group
+#pragma unroll
+                for (int i = 0; i < MT; i++) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        if (2 * i + h >= H) continue;
+                        const float2 f = W4Type<T>::unpack2(sz[(i * 16 + h * 8) * PITCH + word / GW]);       // scale, zero point (+ magic)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const int k = 2 * h + e;
+                            const float sum = kHalf ? fmaf(acc[i][k], 16777216.f, acc_hi[i][k] * 1048576.f) : acc[i][k];
+                            y[i][k] = fmaf(f.x, fmaf(-f.y, gs[e], sum), y[i][k]);
+                        }
+                    }
+                }
+            }
+        }
+    };
+    int at = 0;                                                    // ring slot of the next block
+    for (int kc = 0; kc < nblocks; kc += kW4ChunkBlocks) {
+        if (kc) __syncthreads();                                   // the last pass over this memory is over
+        stage_scales(kc);
+        __syncthreads();
+        const int end = nblocks - kc < kW4ChunkBlocks ? nblocks : kc + kW4ChunkBlocks;
+        const uint32_t* sz = s_sz + g * PITCH + warp * G;
+        // a warp's first block of this chunk: kW4ChunkBlocks need not be a multiple of W
+        int kb = kc + ((warp - kc) % W + W) % W;
+        sz += (kb - kc - warp) * G;
+#pragma unroll 1
+        for (; kb < end; kb += W, sz += W * G) {
+            uint4 b[4];
+            load_b(b, kb);
+            fetch(at ? at - 1 : kW4Depth - 1, kb + (kW4Depth - 1) * W);                    // into the slot read a step ago
+            copy_wait<kW4Depth - 1>();
+            block(ring + at * STEP_BYTES, b, sz);
+            at = at + 1 == kW4Depth ? 0 : at + 1;
+        }
+    }
+    // the warps' sums, in a fixed order
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (2 * i + (e >> 1) < H) red[warp][2 * t + (e & 1)][i * 16 + g + 8 * (e >> 1)] = y[i][e];
+    __syncthreads();
+    for (int o = threadIdx.x; o < 8 * ROWS; o += W * 32) {
+        const int n = o / ROWS, m = o % ROWS;
+        if (n < count && row0 + m < p.M) {
+            float v = 0.f;
+#pragma unroll
+            for (int q = 0; q < W; q++) v += red[q][n][m];
+            if (p.rows) {
+                const int src = p.rows[first + n];
+                if (src < 0 || src >= p.x_rows) v = 0.f;
+            }
+            static_cast<uint16_t*>(p.out)[(long long)(first + n) * p.out_ld + row0 + m] = W4Type<T>::from_float(v);
         }
     }
 }
 
-template <typename T, int W, int H, int NTL, int GW>
+template <typename T, int W, int H, int GW>
 static int stream_launch(cudaStream_t stream, const W4Gemm& p, dim3 grid) {
     constexpr int ROWS = H * 8;
-    constexpr int scale_bytes = ROWS * w4_pitch<GW>() * 4, sum_bytes = W * NTL * 8 * (ROWS + 4) * 4;
+    constexpr int scale_bytes = ROWS * w4_pitch<GW>() * 4, sum_bytes = W * 8 * (ROWS + 4) * 4;
     constexpr int bytes = W * kW4Depth * ROWS * kW4BlockBytes + (scale_bytes > sum_bytes ? scale_bytes : sum_bytes);
     static_assert(bytes <= 227 * 1024, "shared memory of a CTA");
     static bool configured[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 64 || !configured[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(w4_stream_kernel<T, W, H, NTL, GW>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        const cudaError_t e = cudaFuncSetAttribute(w4_stream_kernel<T, W, H, GW>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
         if (e != cudaSuccess) return (int)e;
         if (dev < 64) configured[dev] = true;
     }
-    const cudaError_t e = launch_pdl_smem(w4_stream_kernel<T, W, H, NTL, GW>, grid, dim3(W * 32), (size_t)bytes, stream, p);
+    const cudaError_t e = launch_pdl_smem(w4_stream_kernel<T, W, H, GW>, grid, dim3(W * 32), (size_t)bytes, stream, p);
     count_launch();
     return (int)(e != cudaSuccess ? e : cudaGetLastError());
 }
-template <typename T, int W, int H, int NTL>
-static int stream_groups(cudaStream_t stream, const W4Gemm& p, long long experts) {
-    const dim3 grid((unsigned)((p.M + H * 8 - 1) / (H * 8)), (unsigned)experts);
-    if (p.group == 32) return stream_launch<T, W, H, NTL, 1>(stream, p, grid);
-    if (p.group == 64) return stream_launch<T, W, H, NTL, 2>(stream, p, grid);
-    return stream_launch<T, W, H, NTL, 4>(stream, p, grid);
+
+// Groups of eight rows at most: each expert may end in a partial one.
+static long long w4_octets(const W4Gemm& p) {
+    if (!p.offsets) return (p.slots + 7) / 8;
+    const long long experts = p.slots < p.E ? p.slots : p.E;
+    return experts + (p.slots - experts) / 8;
+}
+
+template <typename T, int W, int H>
+static int stream_groups(cudaStream_t stream, const W4Gemm& p) {
+    const dim3 grid((unsigned)((p.M + H * 8 - 1) / (H * 8)), (unsigned)w4_octets(p));
+    if (p.group == 32) return stream_launch<T, W, H, 1>(stream, p, grid);
+    if (p.group == 64) return stream_launch<T, W, H, 2>(stream, p, grid);
+    return stream_launch<T, W, H, 4>(stream, p, grid);
 }
 
 // Warps and rows of a CTA. The launch lasts as long as the SM with the most rows (a tile more than an SM's share is a seventh
@@ -337,18 +354,14 @@ static int stream_groups(cudaStream_t stream, const W4Gemm& p, long long experts
 // 4 x 40 9.24, 8 x 16 10.3; 14336 x 4096 4 x 40 11.0, 4 x 32 11.2, 8 x 40 13.1.
 template <typename T>
 static int stream_variant(cudaStream_t stream, const W4Gemm& p) {
-    const long long experts = p.offsets ? (p.slots < p.E ? p.slots : p.E) : 1, sms = sm_count();
-    const auto tiles = [&](int rows) { return (p.M + rows - 1) / rows * experts; };
+    const long long octets = p.offsets ? (p.slots < p.E ? p.slots : p.E) : (p.slots + 7) / 8, sms = sm_count();
+    const auto tiles = [&](int rows) { return (p.M + rows - 1) / rows * octets; };
     const auto most_rows = [&](int rows) { return (tiles(rows) + sms - 1) / sms * rows; };
-    if (p.slots > 8 * experts) {          // two column tiles a pass (4096 x 4096 on 16 rows: 8 x 16 7.7, 4 x 32 8.7; 28672 x 8192: 63, 53)
-        if (tiles(16) <= 2 * sms) return stream_groups<T, 8, 2, 2>(stream, p, experts);
-        return stream_groups<T, 4, 4, 2>(stream, p, experts);
-    }
-    if (tiles(16) <= sms) return stream_groups<T, 12, 2, 1>(stream, p, experts);
-    if (tiles(16) <= 2 * sms) return stream_groups<T, 8, 2, 1>(stream, p, experts);
+    if (tiles(16) <= sms) return stream_groups<T, 12, 2>(stream, p);
+    if (tiles(16) <= 2 * sms) return stream_groups<T, 8, 2>(stream, p);
     const bool forty = most_rows(40) < most_rows(32), shared = 2 * tiles(32) <= 5 * sms;
-    if (shared) return forty ? stream_groups<T, 8, 5, 1>(stream, p, experts) : stream_groups<T, 8, 4, 1>(stream, p, experts);
-    return forty ? stream_groups<T, 4, 5, 1>(stream, p, experts) : stream_groups<T, 4, 4, 1>(stream, p, experts);
+    if (shared) return forty ? stream_groups<T, 8, 5>(stream, p) : stream_groups<T, 8, 4>(stream, p);
+    return forty ? stream_groups<T, 4, 5>(stream, p) : stream_groups<T, 4, 4>(stream, p);
 }
 
 int launch_w4_stream(cudaStream_t stream, const W4Gemm& p, int dtype) {

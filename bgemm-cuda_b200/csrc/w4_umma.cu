@@ -149,9 +149,12 @@ struct UPlan {
     __device__ __forceinline__ int total() const { return tiles[E] * mpairs * splits; }
     __device__ __forceinline__ UTile get(int t) const {
         UTile r;
-        r.split = t % splits;
-        t /= splits;
-        const int rt = t % mpairs, tt = t / mpairs;
+        r.split = 0;
+        if (splits > 1) {
+            r.split = t % splits;
+            t /= splits;
+        }
+        const int tt = (int)((unsigned)t / (unsigned)mpairs), rt = t - tt * mpairs;
         int lo = 0, hi = E;           // tiles[lo] <= tt < tiles[hi]
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
@@ -166,8 +169,12 @@ struct UPlan {
         r.valid = count - at < step ? count - at : step;
         r.n = (r.valid + 31) & ~31;
         r.m0 = rt * 256;
-        r.kb0 = (int)((long long)nkb * r.split / splits);
-        r.kb1 = (int)((long long)nkb * (r.split + 1) / splits);
+        r.kb0 = 0;
+        r.kb1 = nkb;
+        if (splits > 1) {
+            r.kb0 = nkb * r.split / splits;              // nkb <= 2^17, splits <= 8
+            r.kb1 = nkb * (r.split + 1) / splits;
+        }
         return r;
     }
 };
@@ -207,7 +214,6 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
     uint64_t* bars = reinterpret_cast<uint64_t*>(misc);
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(misc + 320);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-    long long* s_cost = reinterpret_cast<long long*>(misc + 384);          // [8]
     int* s_first = reinterpret_cast<int*>(misc + 512);
     int* s_tiles = s_first + kUMaxExperts + 8;
 
@@ -246,7 +252,7 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
     }
     grid_dependency_wait();
 
-    // ---- the plan: counts of the experts, tile width, prefix sums ----
+    // ---- the plan, by one warp: the experts' ranges, the tile width, prefix sums of the tiles ----
     const int E = p.g.E;
     if (warp == 1) {
         int carry = 0;                                   // ranges are made ascending and kept inside [0, slots]
@@ -263,32 +269,43 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
             if (e <= E) s_first[e] = v;
             carry = __shfl_sync(0xffffffffu, v, 31);
         }
-    }
-    __syncthreads();
-    if (warp < 8) {                                      // candidate widths 32, 64 .. 256
-        const int nt = 32 * (warp + 1);
-        int tiles = 0;
-        for (int e = lane; e < E; e += 32) tiles += (s_first[e + 1] - s_first[e] + nt - 1) / nt;
+        __syncwarp();
+        // candidate widths 32, 64 .. 256; lane c of the first eight works out the cost of 32 (c + 1)
+        int tiles[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        for (int e = lane; e < E; e += 32) {
+            const unsigned n = (unsigned)(s_first[e + 1] - s_first[e]);
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, d);
-        if (lane == 0) {
-            const long long rounds = ((long long)tiles * p.mpairs * p.splits + ncl - 1) / ncl;
-            // clocks of a tile: 4 per column and 128-column block of tensor work, ~360 per block for the codes at this SM's share
-            // of the memory, and a fixed part for filling the pipeline and draining the accumulator
-            const long long per_block = 4 * nt > 360 ? 4 * nt : 360;
-            s_cost[warp] = rounds * (per_block * ((nkb + p.splits - 1) / p.splits) + 2000 + 6 * nt);
+            for (int c = 0; c < 8; c++) tiles[c] += (int)((n + 32 * c + 31) / (32 * c + 32));
         }
-    }
-    __syncthreads();
-    if (warp == 1) {
-        int best = 7;
-        for (int c = 6; c >= 0; c--)
-            if (s_cost[c] < s_cost[best]) best = c;
-        const int nt = 32 * (best + 1);
-        int carry = 0;
+        int mine = 0;
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) tiles[c] += __shfl_xor_sync(0xffffffffu, tiles[c], d);
+            if (lane == c) mine = tiles[c];
+        }
+        // clocks of a tile: 4 per column and 128-column block of tensor work, ~700 per block for the codes and their unpacking,
+        // and a fixed part for filling the pipeline and draining the accumulator
+        const int nt = 32 * (lane + 1);
+        const float rounds = ceilf((float)mine * (float)(p.mpairs * p.splits) / (float)ncl);
+        const float per_block = 4 * nt > 700 ? (float)(4 * nt) : 700.f;
+        float cost = rounds * (per_block * (float)((nkb + p.splits - 1) / p.splits) + 2000.f + 6.f * (float)nt);
+        int best = lane < 8 ? lane : 7;
+        if (lane >= 8) cost = 3.0e38f;
+#pragma unroll
+        for (int d = 4; d > 0; d >>= 1) {                // the least cost; of equal ones the wider tile
+            const float oc = __shfl_xor_sync(0xffffffffu, cost, d);
+            const int ob = __shfl_xor_sync(0xffffffffu, best, d);
+            if (oc < cost || (oc == cost && ob > best)) {
+                cost = oc;
+                best = ob;
+            }
+        }
+        const unsigned width = 32u * (unsigned)(__shfl_sync(0xffffffffu, best, 0) + 1);
+        carry = 0;
         for (int base = 0; base < E; base += 32) {
             const int e = base + lane;
-            const int x = e < E ? (s_first[e + 1] - s_first[e] + nt - 1) / nt : 0;
+            const int x = e < E ? (int)(((unsigned)(s_first[e + 1] - s_first[e]) + width - 1) / width) : 0;
             int s = x;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
