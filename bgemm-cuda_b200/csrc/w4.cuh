@@ -52,6 +52,15 @@ struct W4Type<__nv_bfloat16> {
     }
 };
 
+template <int DT>
+struct W4OfDtype {
+    using type = __half;
+};
+template <>
+struct W4OfDtype<BGEMM_DT_BF16> {
+    using type = __nv_bfloat16;
+};
+
 // (v & mask) | magic in ONE logic instruction. Written as C the two constants would be two immediates, of which an
 // instruction can hold one, and the compiler splits it.
 __device__ __forceinline__ uint32_t w4_field(uint32_t v, uint32_t mask, uint32_t magic) {

@@ -6,8 +6,9 @@
 // r16 rounds to the scales' 16-bit type (nearest even), everything else is 32-bit arithmetic, rint rounds ties to even.
 //
 // Both kernels are bound by memory: 2 (4) bytes in and half a byte out per weight, or the reverse. A lane owns 8 consecutive
-// columns -- one 16-byte load and one word of codes -- sixteen lanes a storage block; the group's extremes are exchanged
-// with 2 to 4 shuffles.
+// columns -- one 16-byte load and one word of codes --, sixteen lanes a storage block; the group's extremes are exchanged with
+// 2 to 4 shuffles. A warp takes 1024 columns of a row at a time, four loads of a lane on their way (one at a time, with a 64-bit
+// division for its place, took 450 us for both kernels on 28672 x 8192 bf16, groups of 64; now 142 + 94, 182 at the copy bandwidth; the way there is bound by its arithmetic, the way back by memory).
 #include <cuda_runtime.h>
 
 #include "internal.h"
@@ -16,101 +17,195 @@
 
 namespace bgemm {
 
+constexpr int kQSteps = 4;                                         // 8-column chunks of a lane in a unit
+constexpr int kQUnit = kQSteps * 32;                               // chunks of a unit: 1024 columns
+
+// Eight columns as they are stored. `piece`: bytes of the widest access that the rows' alignment allows (16, 8, 4 or 2).
 template <int DT>
-__device__ __forceinline__ void load8(const void* src, long long at, int valid, bool vec, float (&v)[8]) {
-    if (valid >= 8 && vec) {
-        if (DT == BGEMM_DT_F32) {
-            const float4 a = __ldcs(reinterpret_cast<const float4*>(static_cast<const float*>(src) + at));
-            const float4 b = __ldcs(reinterpret_cast<const float4*>(static_cast<const float*>(src) + at + 4));
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-            const uint4 a = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(src) + at));
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+struct Raw8 {
+    uint32_t r[DT == BGEMM_DT_F32 ? 8 : 4];
+};
+template <int DT>
+__device__ __forceinline__ void load8(Raw8<DT>& v, const void* src, long long at, int valid, int piece) {
+    constexpr int N = DT == BGEMM_DT_F32 ? 8 : 4;
+    const uint32_t* p = DT == BGEMM_DT_F32 ? static_cast<const uint32_t*>(src) + at : reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(src) + at);
+    if (valid >= 8 && piece == 16) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float2 f = DT == BGEMM_DT_F16 ? W4Type<__half>::unpack2(w[i]) : W4Type<__nv_bfloat16>::unpack2(w[i]);
-                v[2 * i] = f.x;
-                v[2 * i + 1] = f.y;
+        for (int i = 0; i < N; i += 4) {
+            const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p + i));
+            v.r[i] = a.x; v.r[i + 1] = a.y; v.r[i + 2] = a.z; v.r[i + 3] = a.w;
+        }
+    } else if (valid >= 8 && piece == 8) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const uint2 a = __ldcs(reinterpret_cast<const uint2*>(p + i));
+            v.r[i] = a.x; v.r[i + 1] = a.y;
+        }
+    } else if (valid >= 8 && piece == 4) {
+#pragma unroll
+        for (int i = 0; i < N; i++) v.r[i] = __ldcs(p + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) v.r[i] = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i < valid) {
+                if (DT == BGEMM_DT_F32) v.r[DT == BGEMM_DT_F32 ? i : 0] = p[i];
+                else v.r[i >> 1] |= (uint32_t)static_cast<const uint16_t*>(src)[at + i] << (16 * (i & 1));
             }
-        }
-        return;
     }
+}
+template <int DT>
+__device__ __forceinline__ void floats8(const Raw8<DT>& v, float (&f)[8]) {
+    if (DT == BGEMM_DT_F32) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        float f = 0.f;
-        if (i < valid) {
-            if (DT == BGEMM_DT_F32) f = static_cast<const float*>(src)[at + i];
-            else if (DT == BGEMM_DT_F16) f = W4Type<__half>::to_float(static_cast<const uint16_t*>(src)[at + i]);
-            else f = W4Type<__nv_bfloat16>::to_float(static_cast<const uint16_t*>(src)[at + i]);
+        for (int i = 0; i < 8; i++) f[i] = __uint_as_float(v.r[DT == BGEMM_DT_F32 ? i : 0]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 p = DT == BGEMM_DT_F16 ? W4Type<__half>::unpack2(v.r[i]) : W4Type<__nv_bfloat16>::unpack2(v.r[i]);
+            f[2 * i] = p.x;
+            f[2 * i + 1] = p.y;
         }
-        v[i] = f;
     }
 }
 
-// rint(w / s) for |w / s| < 2^20, without a division per element. r = rint(w * (1 / s)) can only be wrong where w / s lies
-// next to a half: e = w - r s is exact there (r s has few bits, and e is a multiple of w's last place no smaller than
-// 2^-24 s), so |e| clearly below s / 2 proves r; the rest (ties, mostly) takes the division.
-__device__ __forceinline__ float quotient_rint(float w, float s, float inv, float near_half) {
-    const float magic = 12582912.f;                                // 1.5 * 2^23: adding it rounds to a whole number, ties to even
-    float r = __fsub_rn(__fadd_rn(__fmul_rn(w, inv), magic), magic);
-    const float e = __fmaf_rn(-r, s, w);
-    if (!(fabsf(e) < near_half)) r = rintf(__fdiv_rn(w, s));
-    return r;
+// The largest -v and the largest v of eight columns and zero, as floats. 16-bit types are compared two at a time.
+template <int DT, int LG>
+__device__ __forceinline__ float2 extremes8(const Raw8<DT>& v) {
+    float down = 0.f, up = 0.f;
+    if (DT == BGEMM_DT_F32) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float f = __uint_as_float(v.r[DT == BGEMM_DT_F32 ? i : 0]);
+            down = fmaxf(down, -f);
+            up = fmaxf(up, f);
+        }
+#pragma unroll
+        for (int d = 1; d < (1 << LG); d <<= 1) {
+            down = fmaxf(down, __shfl_xor_sync(0xffffffffu, down, d));
+            up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, d));
+        }
+        return make_float2(down, up);
+    }
+    using X = typename W4OfDtype<DT>::type;
+    using T2 = typename W4Type<X>::T2;
+    const auto as2 = [](uint32_t u) { return *reinterpret_cast<const T2*>(&u); };
+    const auto bits = [](T2 h) { return *reinterpret_cast<const uint32_t*>(&h); };
+    const T2 m = __hmax2(__hmax2(as2(v.r[0]), as2(v.r[1])), __hmax2(as2(v.r[2]), as2(v.r[3])));
+    const T2 n = __hmax2(__hmax2(__hneg2(as2(v.r[0])), __hneg2(as2(v.r[1]))), __hmax2(__hneg2(as2(v.r[2])), __hneg2(as2(v.r[3]))));
+    T2 both = __hmax2(as2(__byte_perm(bits(n), bits(m), 0x5410)), as2(__byte_perm(bits(n), bits(m), 0x7632)));      // (-lowest, highest)
+    both = __hmax2(both, as2(0u));
+#pragma unroll
+    for (int d = 1; d < (1 << LG); d <<= 1) both = __hmax2(both, as2(__shfl_xor_sync(0xffffffffu, bits(both), d)));
+    return W4Type<X>::unpack2(bits(both));
 }
 
-template <int DT, typename S>
-__global__ void __launch_bounds__(256) w4_quantize_kernel(const void* __restrict__ src, long long M, int K, long long ld, int lanes_log2 /*lanes per group: 4, 8, 16*/,
-                                                          int symmetric, uint32_t* __restrict__ plane, uint16_t* __restrict__ scales,
-                                                          uint8_t* __restrict__ zeros, long long batch_stride, int vec) {
+__device__ __forceinline__ float pick8(const float (&v)[8], int i) {
+    float f = v[0];
+#pragma unroll
+    for (int j = 1; j < 8; j++) f = j == i ? v[j] : f;
+    return f;
+}
+
+// rint(w / s), inv = 1 / s to a place or two. The quotient is corrected once by its exact remainder (P. Markstein, "Computation of
+// elementary functions on the IBM RISC System/6000 processor", 1990), after which it is off by less than 2^-44 before its own
+// rounding: where w / s is exactly a half it is that half, and two numbers of 11 bits that do not divide to a half stay 2^-22
+// away from one, so the whole number is the division's own. (A test of |w - r s| against s / 2 that sends only doubtful octets to
+// a division took 259 us on 28672 x 8192 bf16: two in five warps held a tie.)
+__device__ __forceinline__ float quotient_rint(float w, float s, float inv) {
+    const float magic = 12582912.f;                                // 1.5 * 2^23: adding it rounds to a whole number, ties to even
+    float t = __fmul_rn(w, inv);
+    t = __fmaf_rn(__fmaf_rn(-t, s, w), inv, t);
+    return __fsub_rn(__fadd_rn(t, magic), magic);
+}
+
+// LG: log2 of the lanes (8 columns each) of a group. SYM: symmetric codes.
+template <int DT, typename S, int LG, bool SYM>
+__global__ void __launch_bounds__(256) w4_quantize_kernel(const void* __restrict__ src, long long M, int K, long long ld, uint32_t* __restrict__ plane,
+                                                          uint16_t* __restrict__ scales, uint8_t* __restrict__ zeros, long long batch_stride, int piece) {
     grid_dependency_wait();
     const int chunks = (K + 127) / 128 * 16;                       // 8-column chunks per row, whole blocks
-    const int half_warps = (chunks + 31) / 32;                     // warp steps per row
-    const int groups = (K + (8 << lanes_log2) - 1) / (8 << lanes_log2);
-    const int lane = threadIdx.x & 31;
+    const unsigned units = (unsigned)(chunks + kQUnit - 1) / kQUnit;
+    const int groups = (K + (8 << LG) - 1) / (8 << LG);
+    const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    const int word_of_lane = (lane >> 4) * 16 + (lane & 3) * 4 + ((lane >> 2) & 3);
     const long long batch = blockIdx.y;
-    const long long steps = M * half_warps, nwarps = (long long)gridDim.x * (blockDim.x >> 5);
+    const long long steps = M * units, nwarps = (long long)gridDim.x * 8;
     const char* base = static_cast<const char*>(src) + batch * batch_stride * (DT == BGEMM_DT_F32 ? 4 : 2);
     plane += batch * M * chunks;
     scales += batch * M * groups;
-    if (zeros) zeros += batch * M * groups;
-    for (long long st = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); st < steps; st += nwarps) {
-        const long long m = st / half_warps;
-        const int chunk = (int)(st - m * half_warps) * 32 + lane;
-        const int k0 = chunk * 8;
-        float v[8];
-        load8<DT>(base, m * ld + k0, K - k0, vec != 0, v);
-        float lo = 0.f, hi = 0.f;
+    if (!SYM) zeros += batch * M * groups;
+    constexpr float magic = 12582912.f;
+    for (long long st = (long long)blockIdx.x * 8 + warp; st < steps; st += nwarps) {
+        // M <= 2^24 rows of at most 2^14 units
+        const long long m = units == 1 ? st : (st < (1LL << 32) ? (long long)((unsigned)st / units) : st / units);
+        const int unit = (int)(st - m * units) * kQUnit;
+        const bool whole = (unit + kQUnit) * 8 <= K && piece == 16;
+        Raw8<DT> raw[kQSteps];
+        const long long at = m * ld + (unit + lane) * 8;
+        if (whole) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            lo = fminf(lo, v[i]);
-            hi = fmaxf(hi, v[i]);
-        }
-        for (int d = 1; d < (1 << lanes_log2); d <<= 1) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
-        }
-        const float range = symmetric ? __fmul_rn(fmaxf(-lo, hi), 1.f / 7.f) : __fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f);
-        const uint16_t s16 = W4Type<S>::from_float(range);
-        const float s = W4Type<S>::to_float(s16);
-        float z = symmetric ? 8.f : 0.f, inv = 0.f;
-        if (s > 0.f) {
-            inv = __fdiv_rn(1.f, s);
-            if (!symmetric) z = fminf(fmaxf(rintf(__fdiv_rn(-lo, s)), 0.f), 15.f);
-        }
-        uint32_t word = 0;
-        const float near_half = s * 0.49999f;
+            for (int q = 0; q < kQSteps; q++) load8<DT>(raw[q], base, at + q * 256, 8, 16);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            float r = s > 0.f ? quotient_rint(v[i], s, inv, near_half) : 0.f;
-            r = fminf(fmaxf(r + z, 0.f), 15.f);
-            word |= (uint32_t)(int)r << (4 * ((i & 1) ? 4 + i / 2 : i / 2));
+            for (int q = 0; q < kQSteps; q++) load8<DT>(raw[q], base, at + q * 256, K - (unit + lane + q * 32) * 8, piece);
         }
-        if (k0 >= K) word = 0;                                     // the padding of the last block
-        if (chunk < chunks) plane[m * chunks + (chunk >> 4) * 16 + (chunk & 3) * 4 + ((chunk >> 2) & 3)] = word;
-        const int g = chunk >> lanes_log2;
-        if ((chunk & ((1 << lanes_log2) - 1)) == 0 && g < groups) {
-            scales[m * groups + g] = s16;
-            if (zeros) zeros[m * groups + g] = (uint8_t)(int)z;
+        uint32_t* out = plane + m * chunks + unit + word_of_lane;
+        const int g0 = (unit + lane) >> LG;
+        uint16_t* s_out = scales + m * groups + g0;
+        uint8_t* z_out = SYM ? nullptr : zeros + m * groups + g0;
+#pragma unroll
+        for (int q = 0; q < kQSteps; q++) {
+            const int chunk = unit + lane + q * 32;
+            if (chunk - lane >= chunks) break;                     // the same for the whole warp
+            const float2 ext = extremes8<DT, LG>(raw[q]);
+            const float range = SYM ? __fmul_rn(fmaxf(ext.x, ext.y), 1.f / 7.f) : __fmul_rn(__fadd_rn(ext.y, ext.x), 1.f / 15.f);
+            const uint16_t s16 = W4Type<S>::from_float(range);
+            const float s = W4Type<S>::to_float(s16);
+            float z = SYM ? 8.f : 0.f;
+            uint32_t word;
+            if (s > 0.f) {
+                const float inv = __fdividef(1.f, s);
+                float v[8], r[8], zr = 0.f;
+                floats8<DT>(raw[q], v);
+                if (s >= 1.2e-38f && s <= 4.0e37f) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) r[i] = quotient_rint(v[i], s, inv);
+                    if (!SYM) zr = quotient_rint(ext.x, s, inv);
+                } else {                                           // 1 / s is not a normal number
+#pragma unroll 1
+                    for (int i = 0; i < 9; i++) {
+                        const float w = i == 8 ? ext.x : pick8(v, i), whole_number = rintf(__fdiv_rn(w, s));
+                        if (i == 8 && !SYM) zr = whole_number;
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            if (j == i) r[j] = whole_number;
+                    }
+                }
+                if (!SYM) z = fminf(zr, 15.f);
+                // q = clamp(r + z, 0, 15). Below, the clamp is void (r(lowest) = -zr, symmetric r >= -7) unless s itself was rounded
+                // far, as a subnormal number, or z was cut; above, both roundings can add up to 16.
+                const float top = 15.f - z;
+                if (s < 6.2e-5f || zr > 15.f) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) r[i] = fminf(fmaxf(r[i], -z), top);
+                }
+                // the nibbles of either half of the word are added up as one number below 2^16
+                float half[2];
+                half[0] = half[1] = magic + z * 4369.f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) half[i & 1] = __fmaf_rn(SYM ? r[i] : fminf(r[i], top), (float)(1 << (4 * (i >> 1))), half[i & 1]);
+                word = __byte_perm(__float_as_uint(half[0]), __float_as_uint(half[1]), 0x5410);
+            } else {
+                word = SYM ? 0x88888888u : 0u;
+            }
+            if (!whole && chunk * 8 >= K) word = 0;                // the padding of the last block
+            if (whole || chunk < chunks) out[q * 32] = word;
+            if ((lane & ((1 << LG) - 1)) == 0 && (whole || g0 + (q << (5 - LG)) < groups)) {
+                s_out[q << (5 - LG)] = s16;
+                if (!SYM) z_out[q << (5 - LG)] = (uint8_t)(int)z;
+            }
         }
     }
 }
@@ -118,47 +213,85 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const void* __restrict
 template <typename T>
 __global__ void __launch_bounds__(256) w4_dequantize_kernel(const uint32_t* __restrict__ plane, long long M, int K, int lanes_log2,
                                                             const uint16_t* __restrict__ scales, const uint8_t* __restrict__ zeros, uint16_t* __restrict__ out,
-                                                            int vec) {
+                                                            int piece) {
     grid_dependency_wait();
     const int chunks = (K + 127) / 128 * 16, used = (K + 7) / 8;
+    const unsigned units = (unsigned)(chunks + kQUnit - 1) / kQUnit;
     const int groups = (K + (8 << lanes_log2) - 1) / (8 << lanes_log2);
-    const long long total = M * used, stride = (long long)gridDim.x * blockDim.x;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += stride) {
-        const long long m = i / used;
-        const int chunk = (int)(i - m * used), g = chunk >> lanes_log2, k0 = chunk * 8;
-        const uint32_t word = __ldcs(plane + m * chunks + (chunk >> 4) * 16 + (chunk & 3) * 4 + ((chunk >> 2) & 3));
-        const auto s2 = w4_splat<T>(scales[m * groups + g]);
-        const auto mz = w4_splat<T>(w4_magic_zero_bits<T>(zeros ? zeros[m * groups + g] : 8u));
-        uint32_t v[4];
+    const int lane = threadIdx.x & 31;
+    const uint32_t magic = w4_opaque(W4Type<T>::kMagic);
+    const long long steps = M * units, nwarps = (long long)gridDim.x * (blockDim.x >> 5);
+    for (long long st = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); st < steps; st += nwarps) {
+        const long long m = units == 1 ? st : (st < (1LL << 32) ? (long long)((unsigned)st / units) : st / units);
+        const int first = (int)(st - m * units) * kQUnit + lane;
+        uint32_t word[kQSteps], s16[kQSteps], z8[kQSteps];
 #pragma unroll
-        for (int p = 0; p < 4; p++) v[p] = w4_pair<T>(word >> (4 * p), mz, s2);
-        uint16_t* dst = out + m * (long long)K + k0;
-        if (vec) {
-            __stcs(reinterpret_cast<uint4*>(dst), make_uint4(v[0], v[1], v[2], v[3]));
-        } else {
+        for (int q = 0; q < kQSteps; q++) {
+            const int chunk = first + q * 32, g = chunk >> lanes_log2;
+            word[q] = s16[q] = 0u;
+            z8[q] = 8u;
+            if (chunk < used) {
+                word[q] = __ldcs(plane + m * chunks + (chunk >> 4) * 16 + (chunk & 3) * 4 + ((chunk >> 2) & 3));
+                s16[q] = __ldg(scales + m * groups + g);
+                if (zeros) z8[q] = __ldg(zeros + m * groups + g);
+            }
+        }
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (k0 + j < K) dst[j] = (uint16_t)(v[j >> 1] >> (16 * (j & 1)));
+        for (int q = 0; q < kQSteps; q++) {
+            const int chunk = first + q * 32, k0 = chunk * 8;
+            if (chunk >= used) break;
+            const auto s2 = w4_splat<T>(s16[q]);
+            const auto mz = w4_splat<T>(w4_magic_zero_bits<T>(z8[q]));
+            uint32_t v[4];
+#pragma unroll
+            for (int p = 0; p < 4; p++) v[p] = w4_pair<T>(word[q] >> (4 * p), mz, s2, magic);
+            uint16_t* dst = out + m * (long long)K + k0;
+            if (k0 + 8 <= K && piece == 16) {
+                __stcs(reinterpret_cast<uint4*>(dst), make_uint4(v[0], v[1], v[2], v[3]));
+            } else if (k0 + 8 <= K && piece == 8) {
+                __stcs(reinterpret_cast<uint2*>(dst), make_uint2(v[0], v[1]));
+                __stcs(reinterpret_cast<uint2*>(dst) + 1, make_uint2(v[2], v[3]));
+            } else if (k0 + 8 <= K && piece == 4) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) __stcs(reinterpret_cast<uint32_t*>(dst) + j, v[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (k0 + j < K) dst[j] = (uint16_t)(v[j >> 1] >> (16 * (j & 1)));
+            }
         }
     }
 }
 
+// the widest of 16, 8, 4 and 2 bytes that divides an address and its steps, OR-ed together
+static int widest_piece(uintptr_t steps) { return steps % 16 == 0 ? 16 : (steps % 8 == 0 ? 8 : (steps % 4 == 0 ? 4 : 2)); }
 static int lanes_log2_of(int group) { return group == 32 ? 2 : (group == 64 ? 3 : 4); }
+static unsigned quant_blocks(long long M, long long K) {
+    const long long steps = M * (((K + 127) / 128 * 16 + kQUnit - 1) / kQUnit), most = (long long)sm_count() * 32;
+    const long long blocks = (steps + 7) / 8;
+    return (unsigned)(blocks < most ? blocks : most);
+}
 
+template <int DT, typename S, int LG, bool SYM>
+static int quantize_launch(cudaStream_t stream, const void* src, long long M, long long K, long long ld, void* plane, void* scales, void* zeros, long long batch,
+                           long long batch_stride) {
+    const size_t size = DT == BGEMM_DT_F32 ? 4 : 2;
+    const int piece = widest_piece(reinterpret_cast<uintptr_t>(src) | (uintptr_t)(M > 1 ? ld * size : 0) | (uintptr_t)(batch > 1 ? batch_stride * size : 0));
+    const cudaError_t e = launch_pdl(w4_quantize_kernel<DT, S, LG, SYM>, dim3(quant_blocks(M, K), (unsigned)batch), dim3(256), stream, src, M, (int)K, ld,
+                                     static_cast<uint32_t*>(plane), static_cast<uint16_t*>(scales), static_cast<uint8_t*>(zeros), batch_stride, piece);
+    count_launch();
+    return (int)(e != cudaSuccess ? e : cudaGetLastError());
+}
 template <int DT, typename S>
 static int quantize_variant(cudaStream_t stream, const void* src, long long M, long long K, long long ld, int group, int symmetric, void* plane,
                             void* scales, void* zeros, long long batch, long long batch_stride) {
-    const size_t size = DT == BGEMM_DT_F32 ? 4 : 2;
-    const int vec = reinterpret_cast<uintptr_t>(src) % 16 == 0 && (ld * size) % 16 == 0 && (batch == 1 || (batch_stride * size) % 16 == 0);
-    const long long steps = M * (((K + 127) / 128 * 16 + 31) / 32);
-    long long blocks = (steps + 7) / 8;
-    const long long most = (long long)sm_count() * 16;
-    if (blocks > most) blocks = most;
-    const cudaError_t e = launch_pdl(w4_quantize_kernel<DT, S>, dim3((unsigned)blocks, (unsigned)batch), dim3(256), stream, src, M, (int)K, ld,
-                                     lanes_log2_of(group), symmetric, static_cast<uint32_t*>(plane), static_cast<uint16_t*>(scales),
-                                     static_cast<uint8_t*>(zeros), batch_stride, vec);
-    count_launch();
-    return (int)(e != cudaSuccess ? e : cudaGetLastError());
+#define BGEMM_W4_LG(LG) \
+    return symmetric ? quantize_launch<DT, S, LG, true>(stream, src, M, K, ld, plane, scales, zeros, batch, batch_stride) \
+                     : quantize_launch<DT, S, LG, false>(stream, src, M, K, ld, plane, scales, zeros, batch, batch_stride)
+    if (group == 32) BGEMM_W4_LG(2);
+    if (group == 64) BGEMM_W4_LG(3);
+    BGEMM_W4_LG(4);
+#undef BGEMM_W4_LG
 }
 
 int launch_w4_quantize(cudaStream_t stream, const void* src, int dtype, long long M, long long K, long long ld, int group, int symmetric,
@@ -177,16 +310,11 @@ int launch_w4_quantize(cudaStream_t stream, const void* src, int dtype, long lon
 
 int launch_w4_dequantize(cudaStream_t stream, const void* plane, long long M, long long K, int group, const void* scales, const void* zeros,
                          int dtype, void* out) {
-    const int vec = K % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
-    long long blocks = (M * ((K + 7) / 8) + 255) / 256;
-    const long long most = (long long)sm_count() * 32;
-    if (blocks > most) blocks = most;
-    const cudaError_t e =
-        dtype == BGEMM_DT_F16
-            ? launch_pdl(w4_dequantize_kernel<__half>, dim3((unsigned)blocks), dim3(256), stream, static_cast<const uint32_t*>(plane), M, (int)K,
-                         lanes_log2_of(group), static_cast<const uint16_t*>(scales), static_cast<const uint8_t*>(zeros), static_cast<uint16_t*>(out), vec)
-            : launch_pdl(w4_dequantize_kernel<__nv_bfloat16>, dim3((unsigned)blocks), dim3(256), stream, static_cast<const uint32_t*>(plane), M, (int)K,
-                         lanes_log2_of(group), static_cast<const uint16_t*>(scales), static_cast<const uint8_t*>(zeros), static_cast<uint16_t*>(out), vec);
+    const int piece = widest_piece(reinterpret_cast<uintptr_t>(out) | (uintptr_t)(M > 1 ? K * 2 : 0));
+    const dim3 grid(quant_blocks(M, K));
+    const auto kernel = dtype == BGEMM_DT_F16 ? w4_dequantize_kernel<__half> : w4_dequantize_kernel<__nv_bfloat16>;
+    const cudaError_t e = launch_pdl(kernel, grid, dim3(256), stream, static_cast<const uint32_t*>(plane), M, (int)K, lanes_log2_of(group),
+                                     static_cast<const uint16_t*>(scales), static_cast<const uint8_t*>(zeros), static_cast<uint16_t*>(out), piece);
     count_launch();
     return (int)(e != cudaSuccess ? e : cudaGetLastError());
 }
