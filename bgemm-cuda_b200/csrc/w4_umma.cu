@@ -284,11 +284,11 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
             for (int d = 16; d > 0; d >>= 1) tiles[c] += __shfl_xor_sync(0xffffffffu, tiles[c], d);
             if (lane == c) mine = tiles[c];
         }
-        // clocks of a tile: 4 per column and 128-column block of tensor work, ~700 per block for the codes and their unpacking,
-        // and a fixed part for filling the pipeline and draining the accumulator
+        // clocks of a tile, as measured: 620 + 2.3 per column for each 128-column block, and a fixed part for filling the pipeline
+        // and draining the accumulator
         const int nt = 32 * (lane + 1);
         const float rounds = ceilf((float)mine * (float)(p.mpairs * p.splits) / (float)ncl);
-        const float per_block = 4 * nt > 700 ? (float)(4 * nt) : 700.f;
+        const float per_block = 620.f + 2.3f * (float)nt;
         float cost = rounds * (per_block * (float)((nkb + p.splits - 1) / p.splits) + 2000.f + 6.f * (float)nt);
         int best = lane < 8 ? lane : 7;
         if (lane >= 8) cost = 3.0e38f;
