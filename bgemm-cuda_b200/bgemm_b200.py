@@ -329,3 +329,126 @@ def linear_forward(weight_f16: torch.Tensor, acts_f16: torch.Tensor, op: int = O
         check(lib.bgemm_linear_forward(_stream(), weight_f16.data_ptr(), acts_f16.data_ptr(), out.data_ptr(), M, N, K, op, out_kind,
                                        out_layout, _ptr(alpha), split_k, ws.data_ptr(), ws.numel()), "bgemm_linear_forward")
     return out
+
+
+# ---- 4-bit weights and expert routing ----
+def _w4_check(plane, scales, zeros, K, group):
+    _require_cuda(plane, scales, zeros)
+    if not (plane.is_contiguous() and scales.is_contiguous() and plane.dtype == torch.uint8 and scales.dtype in (torch.float16, torch.bfloat16)):
+        raise ValueError("plane (uint8) and scales (float16 or bfloat16) must be contiguous")
+    if K < 1 or plane.shape[-1] != lib.bgemm_w4_row_bytes(K) or scales.shape != plane.shape[:-1] + (-(-K // group),):
+        raise ValueError("plane must be [.., M, w4_row_bytes(K)] and scales [.., M, ceil(K / group)]")
+    if zeros is not None and not (zeros.is_contiguous() and zeros.dtype == torch.uint8 and zeros.shape == scales.shape):
+        raise ValueError("zeros must be contiguous uint8 of the scales' shape")
+
+
+def _rows(x):
+    """(tensor with unit column stride, its row pitch in elements)"""
+    if x.stride(-1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        x = x.contiguous()
+    return x, (x.stride(0) if x.shape[0] > 1 else x.shape[1])
+
+
+def w4_quantize(w: torch.Tensor, group: int = 128, symmetric: bool = False, scale_dtype: "torch.dtype | None" = None):
+    """[M, K] or [B, M, K] weights -> (plane uint8 [.., M, row bytes], scales [.., M, groups], zeros uint8 like scales | None)."""
+    _require_cuda(w)
+    if w.dim() not in (2, 3) or w.numel() == 0:
+        raise ValueError("expected a non-empty [M, K] or [B, M, K] tensor")
+    if w.stride(-1) != 1 or (w.shape[-2] > 1 and w.stride(-2) < w.shape[-1]):
+        w = w.contiguous()
+    M, K = w.shape[-2:]
+    B = w.shape[0] if w.dim() == 3 else 1
+    kind = scale_dtype or (torch.float16 if w.dtype == torch.float32 else w.dtype)
+    lead = tuple(w.shape[:-1])
+    plane = torch.empty(lead + (lib.bgemm_w4_row_bytes(K),), dtype=torch.uint8, device=w.device)
+    scales = torch.empty(lead + (-(-K // group),), dtype=kind, device=w.device)
+    zeros = None if symmetric else torch.empty(scales.shape, dtype=torch.uint8, device=w.device)
+    with torch.cuda.device(w.device):
+        check(lib.bgemm_w4_quantize(_stream(), w.data_ptr(), dtype_code(w), M, K, w.stride(-2) if M > 1 else K, group, 1 if symmetric else 0, _DT[kind],
+                                    plane.data_ptr(), scales.data_ptr(), _ptr(zeros), B, w.stride(0) if B > 1 else 0), "bgemm_w4_quantize")
+    return plane, scales, zeros
+
+
+def w4_dequantize(plane: torch.Tensor, scales: torch.Tensor, zeros: "torch.Tensor | None", K: int, group: int = 128) -> torch.Tensor:
+    _w4_check(plane, scales, zeros, K, group)
+    out = torch.empty(tuple(plane.shape[:-1]) + (K,), dtype=scales.dtype, device=plane.device)
+    with torch.cuda.device(plane.device):
+        check(lib.bgemm_w4_dequantize(_stream(), plane.data_ptr(), out.numel() // K, K, group, scales.data_ptr(), _ptr(zeros), dtype_code(scales),
+                                      out.data_ptr()), "bgemm_w4_dequantize")
+    return out
+
+
+def w4a16_gemm(x: torch.Tensor, plane: torch.Tensor, scales: torch.Tensor, zeros: "torch.Tensor | None" = None, group: int = 128,
+               out: "torch.Tensor | None" = None) -> torch.Tensor:
+    """x [N, K] (the scales' type) times a 4-bit matrix -> [N, M]; `out`: a row-major [N, M] tensor, any row pitch."""
+    _w4_check(plane, scales, zeros, x.shape[1], group)
+    if not x.is_cuda or x.dtype != scales.dtype or plane.dim() != 2:
+        raise ValueError("x must be a CUDA tensor [N, K] of the scales' type and the plane [M, bytes]")
+    x, ld = _rows(x)
+    N, M = x.shape[0], plane.shape[0]
+    if out is None:
+        out = torch.empty((N, M), dtype=x.dtype, device=x.device)
+    elif out.shape != (N, M) or out.dtype != x.dtype or out.stride(1) != 1 or out.device != x.device:
+        raise ValueError("out must be a row-major [N, M] tensor of x's type")
+    need = lib.bgemm_w4a16_workspace_bytes(1, M, x.shape[1], N)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    with torch.cuda.device(x.device):
+        check(lib.bgemm_w4a16_gemm(_stream(), plane.data_ptr(), M, x.shape[1], group, scales.data_ptr(), _ptr(zeros), x.data_ptr(), ld, dtype_code(x), N,
+                                   out.data_ptr(), out.stride(0) if N > 1 else M, _ptr(ws), need), "bgemm_w4a16_gemm")
+    return out
+
+
+def w4a16_grouped_gemm(x: torch.Tensor, plane: torch.Tensor, scales: torch.Tensor, zeros: "torch.Tensor | None", offsets: torch.Tensor,
+                       rows: "torch.Tensor | None" = None, group: int = 128, out: "torch.Tensor | None" = None) -> torch.Tensor:
+    """The same product by expert (plane [E, M, bytes], offsets int32 [E + 1]); rows of the result behind offsets[E] are not written."""
+    _w4_check(plane, scales, zeros, x.shape[1], group)
+    _require_cuda(x, offsets, rows)
+    E, M = plane.shape[0], plane.shape[1]
+    if x.dtype != scales.dtype or plane.dim() != 3 or offsets.dtype != torch.int32 or offsets.numel() != E + 1 or not offsets.is_contiguous():
+        raise ValueError("x must have the scales' type, the plane [E, M, bytes] and offsets int32 [E + 1]")
+    if rows is not None and (rows.dtype != torch.int32 or rows.dim() != 1 or not rows.is_contiguous()):
+        raise ValueError("rows must be a contiguous int32 tensor")
+    x, ld = _rows(x)
+    slots = x.shape[0] if rows is None else rows.numel()
+    if out is None:
+        out = torch.empty((slots, M), dtype=x.dtype, device=x.device)
+    elif out.shape != (slots, M) or out.dtype != x.dtype or out.stride(1) != 1 or out.device != x.device:
+        raise ValueError("out must be a row-major [slots, M] tensor of x's type")
+    need = lib.bgemm_w4a16_workspace_bytes(E, M, x.shape[1], slots)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    with torch.cuda.device(x.device):
+        check(lib.bgemm_w4a16_grouped_gemm(_stream(), plane.data_ptr(), E, M, x.shape[1], group, scales.data_ptr(), _ptr(zeros), x.data_ptr(), x.shape[0], ld,
+                                           dtype_code(x), offsets.data_ptr(), _ptr(rows), slots, out.data_ptr(), out.stride(0) if slots > 1 else M, _ptr(ws),
+                                           need), "bgemm_w4a16_grouped_gemm")
+    return out
+
+
+def moe_route(logits: torch.Tensor, top_k: int, renormalize: bool = True):
+    """[T, E] -> (weights fp32 [T, k], experts int32 [T, k], offsets int32 [E + 1], rows int32 [T k], slots int32 [T, k])."""
+    _require_cuda(logits)
+    x, ld = _rows(logits)
+    T, E = x.shape
+    ints = dict(dtype=torch.int32, device=x.device)
+    weights = torch.empty((T, top_k), dtype=torch.float32, device=x.device)
+    experts, slots = torch.empty((T, top_k), **ints), torch.empty((T, top_k), **ints)
+    offsets, rows = torch.empty(E + 1, **ints), torch.empty(T * top_k, **ints)
+    need = lib.bgemm_moe_route_workspace_bytes(T, E)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    with torch.cuda.device(x.device):
+        check(lib.bgemm_moe_route(_stream(), x.data_ptr(), dtype_code(x), T, E, ld, top_k, 1 if renormalize else 0, weights.data_ptr(), experts.data_ptr(),
+                                  offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(), _ptr(ws), need), "bgemm_moe_route")
+    return weights, experts, offsets, rows, slots
+
+
+def moe_combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor) -> torch.Tensor:
+    """out[t] = sum_j weights[t, j] * y[slots[t, j]]."""
+    _require_cuda(y, slots, weights)
+    if slots.dtype != torch.int32 or weights.dtype != torch.float32 or slots.shape != weights.shape or not (slots.is_contiguous() and weights.is_contiguous()):
+        raise ValueError("slots (int32) and weights (float32) must be contiguous tensors of one shape [T, k]")
+    y, ld = _rows(y)
+    T, M = slots.shape[0], y.shape[1]
+    out = torch.empty((T, M), dtype=y.dtype, device=y.device)
+    with torch.cuda.device(y.device):
+        check(lib.bgemm_moe_combine(_stream(), y.data_ptr(), dtype_code(y), y.shape[0], M, ld, slots.data_ptr(), weights.data_ptr(), T, slots.shape[1],
+                                    out.data_ptr(), M), "bgemm_moe_combine")
+    return out

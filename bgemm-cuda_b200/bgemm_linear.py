@@ -11,7 +11,8 @@ What differs from the reference, on purpose:
   * ``NNLinear_elastic_signed`` (binary weight x ternary activation, pure torch in the reference,
     bgemm_linear.py:246-275) runs on the GPU kernel as well;
   * ``BinaryLinear`` / ``BinaryMLP`` / ``bgemm_attn_matmul_batched`` are additions: prepacked weights,
-    fused per-channel scale, batched heads.
+    fused per-channel scale, batched heads; ``W4Linear`` / ``W4Experts`` too: layers of the same library with
+    4-bit weights and group scales, for what one bit is too few for, alone and as the experts of a mixture.
 """
 from __future__ import annotations
 
@@ -25,6 +26,7 @@ import lowbit_kernel
 __all__ = [
     "BNNLinear", "BGEMMLinear", "BGEMMLinear_elastic_signed", "bgemm_matmul", "bgemm_attn_matmul",
     "BGEMMLinear_bireal", "NNLinear_elastic_signed", "BinaryLinear", "BinaryMLP", "bgemm_attn_matmul_batched",
+    "W4Linear", "W4Experts",
 ]
 
 AND_POP, XOR_POP, ATTN_MM, BWTA = 0, 1, 2, 3
@@ -504,3 +506,89 @@ class BinaryMLP(nn.Module):
         static_x.copy_(x)
         g.replay()
         return static_y.clone()
+
+
+# --------------------------------------------------------------------------------------------------
+# additions: 4-bit weights with group scales
+# --------------------------------------------------------------------------------------------------
+class W4Linear(nn.Module):
+    """Inference layer with 4-bit weights: y = x @ W.T (+ bias), W[m, k] = (q - z) * s with a scale (and, unless symmetric,
+    a zero point) per row and group of ``group_size`` (32, 64 or 128) columns.
+
+    ``weight`` [out, in] is quantised once, on the GPU (fp16 or bf16: the layer then takes and returns that type; fp32 weights
+    make an fp16 layer, or a bf16 one with ``dtype=torch.bfloat16``). Any sizes; any number of rows: up to eight the product is a
+    weight-streaming kernel that never rounds a weight, from a few dozen on the tensor cores take it (csrc/w4_stream.cu,
+    csrc/w4_umma.cu). Forward only: calling it while a gradient is asked of x raises.
+
+    Buffers: ``plane`` (codes, include/bgemm_b200.h has the layout), ``scales``, ``zeros`` (absent when symmetric), ``bias``.
+    """
+
+    def __init__(self, weight: torch.Tensor, group_size: int = 128, symmetric: bool = False, bias: "torch.Tensor | None" = None,
+                 dtype: "torch.dtype | None" = None):
+        super().__init__()
+        if weight.dim() != 2:
+            raise ValueError("W4Linear: weight must be [out_features, in_features]")
+        self.out_features, self.in_features = weight.shape
+        self.group_size, self.symmetric = group_size, symmetric
+        plane, scales, zeros = _w4_quantize(weight, group_size, symmetric, dtype)
+        self.register_buffer("plane", plane)
+        self.register_buffer("scales", scales)
+        self.register_buffer("zeros", zeros)
+        self.register_buffer("bias", None if bias is None else bias.detach().to(scales.dtype).to(scales.device).clone())
+
+    def dequantized(self) -> torch.Tensor:
+        """The weights the codes stand for, [out_features, in_features]."""
+        return lowbit_kernel.w4_dequantize(self.plane, self.scales, self.zeros, self.in_features, self.group_size)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        lead = x.shape[:-1]
+        out = lowbit_kernel.w4a16_linear_forward(x.reshape(-1, self.in_features), self.plane, self.scales, self.zeros, self.group_size)
+        out = out.reshape(*lead, self.out_features)
+        return out if self.bias is None else out + self.bias
+
+
+def _w4_quantize(weight, group_size, symmetric, dtype):
+    w = weight.detach()
+    if dtype is not None and w.dtype != torch.float32 and w.dtype != dtype:
+        w = w.float()                          # the scales take dtype; the codes come from the values as they are
+    return lowbit_kernel.w4_quantize(w, group_size, symmetric, dtype == torch.bfloat16)
+
+
+class W4Experts(nn.Module):
+    """The experts of a mixture with 4-bit weights: for each token t and its top_k experts e with weights p,
+
+        out[t] = sum_e p[t, e] * down_e(silu(gate_e x[t]) * up_e x[t])
+
+    ``gate_up`` [E, 2 I, H] (gate rows first) and ``down`` [E, H, I] are quantised once like W4Linear's weight. ``forward``
+    takes the tokens [.., H] and the router's logits [.., E]: routing, both products and the weighted sum stay on the device, nothing is
+    read back, so a captured forward can be replayed with other tokens. Experts whose logit is -inf are never chosen; a token whose
+    logits are all -inf (padding) gets zeros and costs nothing. Forward only.
+    """
+
+    def __init__(self, gate_up: torch.Tensor, down: torch.Tensor, top_k: int, renormalize: bool = True, group_size: int = 128,
+                 symmetric: bool = False, dtype: "torch.dtype | None" = None):
+        super().__init__()
+        if gate_up.dim() != 3 or down.dim() != 3 or gate_up.shape[0] != down.shape[0] or gate_up.shape[1] != 2 * down.shape[2] or gate_up.shape[2] != down.shape[1]:
+            raise ValueError("W4Experts: gate_up must be [E, 2 I, H] and down [E, H, I]")
+        self.num_experts, self.hidden_size, self.intermediate_size = down.shape
+        if not 1 <= top_k <= min(self.num_experts, 32):
+            raise ValueError("W4Experts: 1 <= top_k <= min(E, 32) required")
+        self.top_k, self.renormalize, self.group_size = top_k, renormalize, group_size
+        for name, w in (("gate_up", gate_up), ("down", down)):
+            plane, scales, zeros = _w4_quantize(w, group_size, symmetric, dtype)
+            self.register_buffer(name + "_plane", plane)
+            self.register_buffer(name + "_scales", scales)
+            self.register_buffer(name + "_zeros", zeros)
+
+    def forward(self, x: torch.Tensor, logits: torch.Tensor) -> torch.Tensor:
+        lead = x.shape[:-1]
+        x2 = x.reshape(-1, self.hidden_size)
+        if logits.shape[:-1] != lead or logits.shape[-1] != self.num_experts:
+            raise ValueError("W4Experts: logits must have x's leading sizes and one value per expert")
+        weights, _, offsets, rows, slots = lowbit_kernel.moe_route(logits.reshape(-1, self.num_experts), self.top_k, self.renormalize)
+        h = lowbit_kernel.w4a16_grouped_forward(x2, self.gate_up_plane, self.gate_up_scales, self.gate_up_zeros, offsets, rows, self.group_size)
+        # rows behind offsets[E] are not written by the products, not read by the next one and named by no slot
+        gate, up = h.split(self.intermediate_size, dim=-1)
+        h = nn.functional.silu(gate) * up
+        y = lowbit_kernel.w4a16_grouped_forward(h, self.down_plane, self.down_scales, self.down_zeros, offsets, None, self.group_size)
+        return lowbit_kernel.moe_combine(y, slots, weights).reshape(*lead, self.hidden_size)
