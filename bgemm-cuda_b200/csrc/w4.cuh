@@ -106,6 +106,7 @@ struct W4Gemm {
     long long row_bytes, x_ld, x_rows, out_ld, slots;
     int E, M, K, groups, group;
     int x_vec;                     // rows of x start on 16-byte boundaries
+    int octet0;                    // streaming kernel: the launch's first group of eight rows
 };
 
 // [first, first + count) of expert e; whatever the offsets hold, the range stays inside [0, slots).

@@ -13,7 +13,7 @@
 // A CTA owns 16 or 32 weight rows; its warps take the 128-column blocks of the rows in turn (adjacent warps
 // read adjacent 64-byte pieces of a row) and their sums meet in shared memory, in a fixed order. Activations are read straight
 // from L1 / L2 in fragment order: there is nothing to stage, no limit on K, and a row index costs nothing.
-// Experts: blockIdx.y counts the experts that have rows; a CTA finds its own in the offsets.
+// blockIdx.y counts the groups of eight rows, of all experts in turn; a CTA finds its own in the offsets.
 #include <cuda_runtime.h>
 
 #include "internal.h"
@@ -21,7 +21,6 @@
 #include "w4.cuh"
 
 namespace bgemm {
-
 
 // 16 bytes from global to shared memory, past L1, waited for by groups.
 __device__ __forceinline__ void copy16(uint32_t dst_smem, const void* src) {
@@ -74,6 +73,7 @@ __device__ __forceinline__ uint4 load_x8(const uint16_t* at, int valid, bool vec
 
 // Columns of one pass over the scales, which wait in shared memory as pairs (scale, zero point) of the 16-bit type.
 constexpr int kW4ChunkBlocks = 64;
+constexpr long long kW4MaxOctets = 65535;                                           // of a launch: blockIdx.y
 constexpr int kW4Depth = 3;                                                         // blocks of a warp on their way, the one at work included
 template <int GW>
 __host__ __device__ constexpr int w4_pitch() { return kW4ChunkBlocks * (4 / GW) + 4; }                  // 4 mod 32, 16-byte rows: the eight rows of a read meet eight banks
@@ -98,7 +98,8 @@ __global__ void __launch_bounds__(W * 32, w4_resident_warps<T>(H) / W) w4_stream
     // the shuffle tells the compiler that the warp's number is uniform: block addresses are then computed by the uniform unit
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), g = lane >> 2, t = lane & 3;
 
-    // This CTA's expert and its eight rows: the blockIdx.y-th group of eight, experts in order.
+    // This CTA's expert and its eight rows: the octet-th group of eight, experts in order.
+    const int octet = p.octet0 + (int)blockIdx.y;
     int expert = 0, first = 0, count;
     if (p.offsets) {
         // lane l looks at experts [l q, (l + 1) q): all loads are on their way at once, one prefix sum over the warp
@@ -116,7 +117,7 @@ __global__ void __launch_bounds__(W * 32, w4_resident_warps<T>(H) / W) w4_stream
             if (lane >= d) before += up;
         }
         before -= mine;
-        const int want = blockIdx.y;
+        const int want = octet;
         const uint32_t has = __ballot_sync(0xffffffffu, want >= before && want < before + mine);
         if (!has) return;
         int found = 0, skip = 0;
@@ -140,7 +141,7 @@ __global__ void __launch_bounds__(W * 32, w4_resident_warps<T>(H) / W) w4_stream
         first += skip;
         count -= skip;
     } else {
-        first = blockIdx.y * 8;
+        first = octet * 8;
         count = (int)p.slots - first;
     }
 
@@ -313,7 +314,7 @@ __global__ void __launch_bounds__(W * 32, w4_resident_warps<T>(H) / W) w4_stream
 }
 
 template <typename T, int W, int H, int GW>
-static int stream_launch(cudaStream_t stream, const W4Gemm& p, dim3 grid) {
+static int stream_launch(cudaStream_t stream, W4Gemm p, long long octets) {
     constexpr int ROWS = H * 8;
     constexpr int scale_bytes = ROWS * w4_pitch<GW>() * 4, sum_bytes = W * 8 * (ROWS + 4) * 4;
     constexpr int bytes = W * kW4Depth * ROWS * kW4BlockBytes + (scale_bytes > sum_bytes ? scale_bytes : sum_bytes);
@@ -326,9 +327,15 @@ static int stream_launch(cudaStream_t stream, const W4Gemm& p, dim3 grid) {
         if (e != cudaSuccess) return (int)e;
         if (dev < 64) configured[dev] = true;
     }
-    const cudaError_t e = launch_pdl_smem(w4_stream_kernel<T, W, H, GW>, grid, dim3(W * 32), (size_t)bytes, stream, p);
-    count_launch();
-    return (int)(e != cudaSuccess ? e : cudaGetLastError());
+    // more groups of eight rows than a grid has places for (half a million rows that TMA cannot take) go in several launches
+    for (long long o = 0; o < octets; o += kW4MaxOctets) {
+        const dim3 grid((unsigned)((p.M + ROWS - 1) / ROWS), (unsigned)(octets - o < kW4MaxOctets ? octets - o : kW4MaxOctets));
+        p.octet0 = (int)o;
+        const cudaError_t e = launch_pdl_smem(w4_stream_kernel<T, W, H, GW>, grid, dim3(W * 32), (size_t)bytes, stream, p);
+        count_launch();
+        if (e != cudaSuccess) return (int)e;
+    }
+    return (int)cudaGetLastError();
 }
 
 // Groups of eight rows at most: each expert may end in a partial one.
@@ -340,10 +347,10 @@ static long long w4_octets(const W4Gemm& p) {
 
 template <typename T, int W, int H>
 static int stream_groups(cudaStream_t stream, const W4Gemm& p) {
-    const dim3 grid((unsigned)((p.M + H * 8 - 1) / (H * 8)), (unsigned)w4_octets(p));
-    if (p.group == 32) return stream_launch<T, W, H, 1>(stream, p, grid);
-    if (p.group == 64) return stream_launch<T, W, H, 2>(stream, p, grid);
-    return stream_launch<T, W, H, 4>(stream, p, grid);
+    const long long octets = w4_octets(p);
+    if (p.group == 32) return stream_launch<T, W, H, 1>(stream, p, octets);
+    if (p.group == 64) return stream_launch<T, W, H, 2>(stream, p, octets);
+    return stream_launch<T, W, H, 4>(stream, p, octets);
 }
 
 // Warps and rows of a CTA. The launch lasts as long as the SM with the most rows (a tile more than an SM's share is a seventh

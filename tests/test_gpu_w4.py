@@ -303,3 +303,20 @@ def test_rows_of_a_stack_beyond_32_bits(L):
         got = L.w4a16_grouped_forward(x[:per].repeat(3, 1), plane, scales, None, ragged(counts), None, group)
         assert torch.equal(got[:per], got[per:2 * per]) and torch.equal(got[:per], got[2 * per:])
         check_linear(got[:per], x[:per], one, s, None, K, group)
+
+
+def test_more_groups_of_eight_rows_than_one_grid_holds():
+    """Rows that TMA cannot take stay on the kernel that gives every eight rows a grid row of their own, of which a launch has
+    65535: half a million rows go in several launches, dense and by expert."""
+    import bgemm_b200 as B
+
+    g = gen(12)
+    M, K, N, group = 3, 9, 65535 * 8 + 4100, 32                            # rows 18 bytes apart
+    plane, scales, zeros = matrix((2,), M, K, group, torch.float16, True, g)
+    x = torch.randn(N, K, generator=g, device="cuda").half()
+    got = B.w4a16_gemm(x, plane[0], scales[0], zeros[0], group)
+    check_linear(got, x, plane[0], scales[0], zeros[0], K, group)
+    cut = 65535 * 8 - 13
+    got = B.w4a16_grouped_gemm(x, plane, scales, zeros, torch.tensor([0, cut, N], dtype=torch.int32, device="cuda"), None, group)
+    check_linear(got[:cut], x[:cut], plane[0], scales[0], zeros[0], K, group)
+    check_linear(got[cut:], x[cut:], plane[1], scales[1], zeros[1], K, group)
