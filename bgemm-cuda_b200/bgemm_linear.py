@@ -541,6 +541,8 @@ class W4Linear(nn.Module):
         return lowbit_kernel.w4_dequantize(self.plane, self.scales, self.zeros, self.in_features, self.group_size)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.dim() < 1 or x.shape[-1] != self.in_features:
+            raise ValueError(f"W4Linear: x must be [.., {self.in_features}]")
         lead = x.shape[:-1]
         out = lowbit_kernel.w4a16_linear_forward(x.reshape(-1, self.in_features), self.plane, self.scales, self.zeros, self.group_size)
         out = out.reshape(*lead, self.out_features)
@@ -548,6 +550,8 @@ class W4Linear(nn.Module):
 
 
 def _w4_quantize(weight, group_size, symmetric, dtype):
+    if dtype not in (None, torch.float16, torch.bfloat16):
+        raise ValueError("4-bit layers: dtype must be torch.float16 or torch.bfloat16")
     w = weight.detach()
     if dtype is not None and w.dtype != torch.float32 and w.dtype != dtype:
         w = w.float()                          # the scales take dtype; the codes come from the values as they are
@@ -581,9 +585,11 @@ class W4Experts(nn.Module):
             self.register_buffer(name + "_zeros", zeros)
 
     def forward(self, x: torch.Tensor, logits: torch.Tensor) -> torch.Tensor:
+        if x.dim() < 1 or x.shape[-1] != self.hidden_size:
+            raise ValueError(f"W4Experts: x must be [.., {self.hidden_size}]")
         lead = x.shape[:-1]
         x2 = x.reshape(-1, self.hidden_size)
-        if logits.shape[:-1] != lead or logits.shape[-1] != self.num_experts:
+        if logits.dim() < 1 or logits.shape[:-1] != lead or logits.shape[-1] != self.num_experts:
             raise ValueError("W4Experts: logits must have x's leading sizes and one value per expert")
         weights, _, offsets, rows, slots = lowbit_kernel.moe_route(logits.reshape(-1, self.num_experts), self.top_k, self.renormalize)
         h = lowbit_kernel.w4a16_grouped_forward(x2, self.gate_up_plane, self.gate_up_scales, self.gate_up_zeros, offsets, rows, self.group_size)

@@ -172,3 +172,17 @@ def test_ctypes_binding_gives_the_same(L):
             call()
     with pytest.raises(B.BgemmError):
         B.moe_route(torch.zeros(2, 8, device="cuda"), 9)
+
+
+def test_layers_refuse_other_widths_and_types(N):
+    """[4, 2 H] is not taken for eight tokens of width H."""
+    g = gen(15)
+    H, I, E = 64, 32, 4
+    gate_up, down = torch.randn(E, 2 * I, H, generator=g, device="cuda").half(), torch.randn(E, H, I, generator=g, device="cuda").half()
+    layer, linear = N.W4Experts(gate_up, down, 2), N.W4Linear(gate_up[0])
+    x, logits = torch.randn(4, 2 * H, generator=g, device="cuda").half(), torch.randn(4, E, generator=g, device="cuda")
+    for call in (lambda: layer(x, logits), lambda: linear(x), lambda: linear(x[:, :32]), lambda: layer(x[:, :H], logits[:3]),
+                 lambda: N.W4Linear(gate_up[0], dtype=torch.float32), lambda: N.W4Experts(gate_up, down, 2, dtype=torch.int8)):
+        with pytest.raises(ValueError):
+            call()
+    assert layer(x[:, :H], logits).shape == (4, H) and linear(x[0, :H]).shape == (2 * I,)
