@@ -111,8 +111,10 @@ size_t bgemm_w4a16_workspace_bytes(int64_t E, int64_t M, int64_t K, int64_t slot
     W4Gemm p{};
     static const int32_t some = 0;
     p.E = (int)E; p.M = (int)M; p.K = (int)K; p.slots = slots; p.x_vec = 1;
-    p.offsets = E > 1 ? &some : nullptr;          // only whether there are any counts here
-    return on_tensor_cores(p) ? w4_umma_workspace(p) : 0;
+    const size_t dense = E == 1 && on_tensor_cores(p) ? w4_umma_workspace(p) : 0;
+    p.offsets = &some;                            // only whether there are any counts here; one matrix may be called either way
+    const size_t grouped = on_tensor_cores(p) ? w4_umma_workspace(p) : 0;
+    return dense > grouped ? dense : grouped;
 }
 
 int bgemm_w4a16_gemm(void* stream, const void* plane, int64_t M, int64_t K, int group, const void* scales, const uint8_t* zeros, const void* x,

@@ -333,6 +333,10 @@ int code16(const torch::Tensor& t, const char* where) {
 
 void check_group(int64_t group, const char* where) { TORCH_CHECK(group == 32 || group == 64 || group == 128, where, ": group_size must be 32, 64 or 128"); }
 
+void no_grad_only(const torch::Tensor& t, const char* where) {
+    TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), where, ": forward only (no gradient): call it under torch.no_grad() or detach its input");
+}
+
 // plane [.., M, row bytes], scales [.., M, groups], zeros the same as scales; all contiguous, on x's device
 void check_w4(const torch::Tensor& plane, const torch::Tensor& scales, const c10::optional<torch::Tensor>& zeros, int64_t K, int64_t group,
               const torch::Device& dev, const char* where) {
@@ -344,16 +348,13 @@ void check_w4(const torch::Tensor& plane, const torch::Tensor& scales, const c10
                 where, ": plane must be [.., M, w4_row_bytes(K)] and scales [.., M, ceil(K / group_size)]");
     for (int64_t d = 0; d + 1 < plane.dim(); d++) TORCH_CHECK(plane.size(d) == scales.size(d), where, ": plane and scales have different shapes");
     code16(scales, where);
+    no_grad_only(scales, where);
     if (zeros.has_value())
         TORCH_CHECK(zeros->device() == dev && zeros->scalar_type() == at::kByte && zeros->is_contiguous() && zeros->sizes() == scales.sizes(), where,
                     ": zeros must be contiguous uint8 of the scales' shape");
 }
 
 uint8_t* zeros_ptr(const c10::optional<torch::Tensor>& zeros) { return zeros.has_value() ? zeros->data_ptr<uint8_t>() : nullptr; }
-
-void no_grad_only(const torch::Tensor& t, const char* where) {
-    TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), where, ": forward only (no gradient): call it under torch.no_grad() or detach its input");
-}
 
 // [M, K] or [E, M, K] weights -> (plane uint8 [.., M, w4_row_bytes(K)], scales [.., M, groups], zeros uint8 [.., M, groups] or None).
 // The scales take the weights' type, fp16 for fp32 weights unless scale_bf16.
@@ -451,6 +452,7 @@ torch::Tensor w4a16_grouped_forward(torch::Tensor x, torch::Tensor plane, torch:
         TORCH_CHECK(out.device() == x.device() && out.scalar_type() == x.scalar_type() && out.dim() == 2 && out.size(0) == slots && out.size(1) == M &&
                         out.stride(1) == 1 && (slots <= 1 || out.stride(0) >= M),
                     where, ": out must be a row-major [slots, M] tensor of x's type and device");
+        no_grad_only(out, where);
     } else {
         out = torch::empty({slots, M}, x.options());
     }

@@ -7,10 +7,10 @@
 //   fp16: a 4-bit field in the low mantissa bits IS the subnormal number q 2^-24, in the next four bits q 2^-20; the two
 //         kinds go to two accumulators and 2^24 / 2^20 joins the scale.
 //   bf16: the product q 2^-133 x would leave the 32-bit range, so the field is OR-ed into 128.0 (128 + q, exact) and
-//         128 joins the zero point.
+//         128 joins the zero point. (143 |x| over 128 columns must stay below 3.4e38: |x| up to 1e34.)
 //   The sums of x over a group, which the zero point needs, come from one more product with a matrix of ones.
 //
-// A CTA owns 16 or 32 weight rows; its warps take the 128-column blocks of the rows in turn (adjacent warps
+// A CTA owns 16, 32 or 40 weight rows; its warps take the 128-column blocks of the rows in turn (adjacent warps
 // read adjacent 64-byte pieces of a row) and their sums meet in shared memory, in a fixed order. Activations are read straight
 // from L1 / L2 in fragment order: there is nothing to stage, no limit on K, and a row index costs nothing.
 // blockIdx.y counts the groups of eight rows, of all experts in turn; a CTA finds its own in the offsets.

@@ -347,8 +347,11 @@ int bgemm_w4_dequantize(void* stream, const void* plane, int64_t M, int64_t K, i
 
 /* y[n, m] = sum_k x[n, k] w[m, k]: x [N, K] (row pitch x_ld elements) and out [N, M] (row pitch out_ld) of `dtype`, which
  * is also the scales' type; sums in 32 bits, rounded once. Any N, M, K and alignment of x.
- * Up to 16 rows the weights enter as the exact products above; beyond (with rows of x on 16-byte boundaries; others take
- * the first path at any N, more slowly) each weight is first rounded to the 16-bit type, as bgemm_w4_dequantize returns it.
+ * Few rows (up to 8 always, up to some dozens where the matrix is small; rows of x off 16-byte boundaries at any N, more
+ * slowly) meet the weights as the exact products above. For more, each weight is first rounded to the 16-bit type, as
+ * bgemm_w4_dequantize returns it: scales so small that (q - z) s is no normal fp16 number lose bits there.
+ * bf16: |x| up to 1e34 (128 columns' sums of (128 + q) x are held in 32 bits before the zero point comes off).
+ * out must not overlap x, the plane or the scales.
  * workspace: optional, bgemm_w4a16_workspace_bytes(1, M, K, N) bytes of any contents, 256-byte aligned: partial sums of
  * launches that have too few tiles to fill the GPU and divide K, and rows of x put together (grouped product, with an
  * index). Without it (or with less) K is not divided and the rows are read by index.
@@ -362,7 +365,8 @@ int bgemm_w4a16_gemm(void* stream, const void* plane, int64_t M, int64_t K, int 
  * [offsets[e], offsets[e + 1]) is multiplied with expert e's matrix: out[s] = W_e x[rows ? rows[s] : s]. `offsets` is a
  * device array int32 [E + 1], ascending from 0 to at most `slots`; experts may be empty; out rows behind offsets[E] are
  * not written. `rows` (device, int32 [slots], or NULL) names the row of x [x_rows, K] a slot reads; an index outside x
- * counts as a row of zeros. workspace as above, bgemm_w4a16_workspace_bytes(E, M, K, slots). The host never reads offsets or rows; whatever they hold, no access leaves the buffers.    */
+ * counts as a row of zeros. workspace as above, bgemm_w4a16_workspace_bytes(E, M, K, slots). The host never reads offsets
+ * or rows; whatever they hold, no access leaves the buffers.                                                            */
 int bgemm_w4a16_grouped_gemm(void* stream, const void* plane, int64_t E, int64_t M, int64_t K, int group, const void* scales,
                              const uint8_t* zeros, const void* x, int64_t x_rows, int64_t x_ld, int dtype, const int32_t* offsets,
                              const int32_t* rows, int64_t slots, void* out, int64_t out_ld, void* workspace,

@@ -320,3 +320,36 @@ def test_more_groups_of_eight_rows_than_one_grid_holds():
     got = B.w4a16_grouped_gemm(x, plane, scales, zeros, torch.tensor([0, cut, N], dtype=torch.int32, device="cuda"), None, group)
     check_linear(got[:cut], x[:cut], plane[0], scales[0], zeros[0], K, group)
     check_linear(got[cut:], x[cut:], plane[1], scales[1], zeros[1], K, group)
+
+
+def test_one_expert_with_an_index_is_the_dense_product(L):
+    """The workspace asked for a single matrix serves the grouped call too: its rows are put together first, and the result is
+    that of the dense call on those rows."""
+    import bgemm_b200 as B
+
+    g = gen(13)
+    M, K, n, group = 4096, 4096, 320, 128
+    plane, scales, zeros = matrix((1,), M, K, group, torch.bfloat16, True, g)
+    x = torch.randn(200, K, generator=g, device="cuda").bfloat16()
+    rows = torch.randint(0, 200, (n,), generator=g, device="cuda", dtype=torch.int32)
+    assert B.lib.bgemm_w4a16_workspace_bytes(1, M, K, n) >= n * K * 2
+    got = L.w4a16_grouped_forward(x, plane, scales, zeros, ragged([n]), rows, group)
+    assert torch.equal(got, L.w4a16_linear_forward(x[rows.long()], plane[0], scales[0], zeros[0], group))
+    check_linear(got, x[rows.long()], plane[0], scales[0], zeros[0], K, group)
+
+
+def test_a_gradient_is_refused_wherever_it_is_asked(L):
+    g = gen(14)
+    plane, scales, zeros = matrix((2,), 16, 64, 64, torch.float16, True, g)
+    x = torch.randn(4, 64, generator=g, device="cuda").half()
+    learnt = scales.clone().requires_grad_(True)
+    out = torch.zeros(4, 16, dtype=torch.float16, device="cuda", requires_grad=True)
+    off = ragged([2, 2])
+    for call in (lambda: L.w4a16_linear_forward(x, plane[0], learnt[0], zeros[0], 64), lambda: L.w4_dequantize(plane, learnt, zeros, 64, 64),
+                 lambda: L.w4a16_grouped_forward(x, plane, learnt, zeros, off, None, 64),
+                 lambda: L.w4a16_grouped_forward(x, plane, scales, zeros, off, None, 64, out)):
+        with pytest.raises(RuntimeError):
+            call()
+    with torch.no_grad():
+        want = L.w4a16_grouped_forward(x, plane, scales, zeros, off, None, 64)
+        assert torch.equal(L.w4a16_grouped_forward(x, plane, learnt, zeros, off, None, 64, out), want)
