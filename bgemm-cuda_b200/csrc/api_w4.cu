@@ -51,7 +51,7 @@ W4Gemm problem(const void* plane, int E, int64_t M, int64_t K, int group, const 
 // Which kernel. The streaming kernel passes over a matrix once for every eight rows that meet it; the tensor-core kernel takes
 // any number of rows in one pass, but needs ~9 us to fill and drain and unpacks codes at less than half the memory's rate.
 // Measured (us, streaming / tensor cores): 4096 x 4096 on 16 rows 8 / 15, on 24 10 / 15, on 32 11 / 15; 11008 x 4096 on 16 rows
-// 16 / 18, on 24 22 / 18; 28672 x 8192 on 8 rows 31 / 51, on 16 58 / 51; 177 x 1720 on 709 rows 8 / 16; 64 experts of 2048 x 4096 on 8
+// 14 / 17, on 24 20 / 17; 8192 x 8192 on 12 rows 19 / 22; 28672 x 8192 on 8 rows 31 / 50, on 16 57 / 50; 177 x 1720 on 709 rows 8 / 16; 64 experts of 2048 x 4096 on 8
 // rows each 72 / 98, on 12 129 / 99; 8 of them on 93 rows 24 / 19. So: by the bytes of all passes, a short row counting as
 // 1536 columns (a CTA's own start and end; 18 experts of 11964 x 128 on 160 rows: 61 / 33). Rows of x off 16-byte
 // boundaries cannot be loaded by TMA and stay on the former.
@@ -66,7 +66,7 @@ bool on_tensor_cores(const W4Gemm& p) {
     const double matrix = (double)p.M * (p.K > 1536 ? (double)p.K : 1536.0) / 2;
     if (!p.offsets) {
         const long long passes = (p.slots + 7) / 8;
-        return passes > 1 && passes * matrix > 45e6;
+        return passes > 1 && passes * matrix > (passes == 2 ? 80e6 : 45e6);
     }
     // the counts are on the device: on average an expert's last pass is not full
     const double experts = (double)(p.slots < p.E ? p.slots : p.E), rows = (double)p.slots / experts;

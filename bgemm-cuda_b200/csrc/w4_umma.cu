@@ -479,18 +479,44 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
             const long long at = ((long long)u.expert * p.g.M + m) * p.g.groups;
             const uint16_t* srow = p.g.scales + at;
             const uint8_t* zrow = p.g.zeros ? p.g.zeros + at : nullptr;
-            uint32_t sc[G], ze[G];
-            auto fetch = [&](int kb) {
+            // The scales (two in a word) and zero points (four) of a block, loaded a block of the set ahead. A lane's row is its own cache
+            // line, so it is the number of loads that costs: one of each where the row's alignment allows it (28672 x 8192 on 16 rows in
+            // groups of 64: 71 -> 61 us, of 32: 106 -> 67).
+            constexpr int SW = (G + 1) / 2;
+            struct Raw { uint32_t s[SW], z; };
+            const bool wide = reinterpret_cast<uintptr_t>(srow) % (2 * G) == 0 && reinterpret_cast<uintptr_t>(zrow) % G == 0;
+            const auto fetch = [&](Raw& v, int kb) {
+                if (kb >= u.kb1) return;
+                const uint16_t* sp = srow + kb * G;
+                const uint8_t* zp = zrow + kb * G;
+                v.z = 0x08080808u;
+                if (G > 1 && wide && (kb + 1) * G <= p.g.groups) {
+                    if constexpr (G == 2) {
+                        v.s[0] = __ldg(reinterpret_cast<const uint32_t*>(sp));
+                        if (zrow) v.z = __ldg(reinterpret_cast<const uint16_t*>(zp));
+                    } else if constexpr (G == 4) {
+                        const uint2 s4 = __ldg(reinterpret_cast<const uint2*>(sp));
+                        v.s[0] = s4.x; v.s[1] = s4.y;
+                        if (zrow) v.z = __ldg(reinterpret_cast<const uint32_t*>(zp));
+                    }
+                    return;
+                }
+                uint32_t sv[G], zv[G];
 #pragma unroll
                 for (int q = 0; q < G; q++) {
-                    int grp = kb * G + q;
-                    if (grp >= p.g.groups) grp = p.g.groups - 1;      // behind K: the activations there are zero
-                    sc[q] = __ldg(srow + grp);
-                    ze[q] = zrow ? __ldg(zrow + grp) : 8u;
+                    const int c = kb * G + q < p.g.groups ? q : p.g.groups - 1 - kb * G;      // behind K: the activations there are zero
+                    sv[q] = __ldg(sp + c);
+                    zv[q] = zrow ? __ldg(zp + c) : 8u;
                 }
+                v.z = 0u;
+#pragma unroll
+                for (int q = 0; q < SW; q++) v.s[q] = sv[2 * q] | (2 * q + 1 < G ? sv[2 * q + 1 < G ? 2 * q + 1 : 0] << 16 : 0u);
+#pragma unroll
+                for (int q = 0; q < G; q++) v.z |= zv[q] << (8 * q);
             };
             int kb = u.kb0 + skip;
-            if (kb < u.kb1) fetch(kb);
+            Raw now{};
+            fetch(now, kb);
             for (; kb < u.kb1 && ok; kb += kUSets, lap++) {
                 const uint32_t ws = wring.slot;
                 ok = mbar_wait(w_full + 8 * ws, wring.full_parity(), abort_flag, p.status, 57);
@@ -507,10 +533,8 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
                 fence_proxy_async_smem();     // generic-proxy reads before the producer's next copy into this stage
                 __syncwarp();
                 if (lane == 0) mbar_arrive(w_empty + 8 * ws);
-                uint32_t s_now[G], z_now[G];
-#pragma unroll
-                for (int q = 0; q < G; q++) { s_now[q] = sc[q]; z_now[q] = ze[q]; }
-                if (kb + kUSets < u.kb1) fetch(kb + kUSets);
+                const Raw cur = now;
+                fetch(now, kb + kUSets);
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
                     // the first half's arithmetic comes before the wait for the stage
@@ -518,8 +542,9 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
 #pragma unroll
                     for (int q = 0; q < 2; q++) {
                         const int w = 2 * half + q;
-                        const auto s2 = w4_splat<T>(s_now[w / GW]);
-                        const auto mz = w4_splat<T>(w4_magic_zero_bits<T>(z_now[w / GW]));
+                        const uint32_t pair = cur.s[w / GW / 2];
+                        const auto s2 = w4_splat<T>(w / GW % 2 ? pair >> 16 : pair & 0xffffu);
+                        const auto mz = w4_splat<T>(w4_magic_zero_bits<T>(cur.z >> (8 * (w / GW))));
                         const uint32_t word[4] = {w == 0 ? c0.x : (w == 1 ? c0.y : (w == 2 ? c0.z : c0.w)), w == 0 ? c1.x : (w == 1 ? c1.y : (w == 2 ? c1.z : c1.w)),
                                                   w == 0 ? c2.x : (w == 1 ? c2.y : (w == 2 ? c2.z : c2.w)), w == 0 ? c3.x : (w == 1 ? c3.y : (w == 2 ? c3.z : c3.w))};
 #pragma unroll
