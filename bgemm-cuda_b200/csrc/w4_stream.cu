@@ -78,15 +78,16 @@ constexpr int kW4Depth = 3;                                                     
 template <int GW>
 __host__ __device__ constexpr int w4_pitch() { return kW4ChunkBlocks * (4 / GW) + 4; }                  // 4 mod 32, 16-byte rows: the eight rows of a read meet eight banks
 
-// Warps an SM is meant to hold. Five octets of fp16 rows spill at what 24 leave each (28672 x 8192 on 8 rows in groups of 64:
-// 47 us, 40 with 20 warps); bf16 does not (31.1, 32.3 with 20).
+// Warps an SM is meant to hold. Registers spill at what 24 leave each with five octets of fp16 rows (28672 x 8192 on 8 rows in
+// groups of 64: 47 us, 40 with 20 warps; bf16 31.1 and 32.3) and with four scale groups a block (in groups of 32: 58 us, 49 with 16; fp16
+// 73 and 56).
 template <typename T>
-__host__ __device__ constexpr int w4_resident_warps(int H) { return H > 4 && W4Type<T>::kMagicValue == 1024.f ? 20 : 24; }
+__host__ __device__ constexpr int w4_resident_warps(int H, int GW) { return GW == 1 && H > 2 ? 16 : (H > 4 && W4Type<T>::kMagicValue == 1024.f ? 20 : 24); }
 
 // W: warps of a CTA (K is divided among them), H: its weight rows in octets (two make a 16-row product, an odd one a product
 // whose other half is zero), GW: 32-column words per scale group (1, 2, 4).
 template <typename T, int W, int H, int GW>
-__global__ void __launch_bounds__(W * 32, w4_resident_warps<T>(H) / W) w4_stream_kernel(const W4Gemm p) {
+__global__ void __launch_bounds__(W * 32, w4_resident_warps<T>(H, GW) / W) w4_stream_kernel(const W4Gemm p) {
     constexpr bool kHalf = W4Type<T>::kMagicValue == 1024.f;
     constexpr int MT = (H + 1) / 2, G = 4 / GW, PITCH = w4_pitch<GW>(), ROWS = H * 8, STEP_BYTES = ROWS * kW4BlockBytes;
     // Per warp a ring of blocks that every lane fills and reads back itself (no barrier anywhere near it), then the scales
@@ -167,11 +168,36 @@ __global__ void __launch_bounds__(W * 32, w4_resident_warps<T>(H) / W) w4_stream
 #pragma unroll
     for (int d = 0; d < kW4Depth - 1; d++) fetch(d, warp + d * W);
 
-    // scales and zero points of the blocks [kb0, kb0 + 64): coalesced along the rows
+    // Scales and zero points of the blocks [kb0, kb0 + 64), coalesced along the rows, two groups of a row a lane (one where the rows
+    // are not aligned to two). The zero point (bf16: 128 + z) is put together from bits: a conversion costs four times an addition.
+    const auto pack_sz = [&](uint32_t s16, uint32_t z) {
+        uint32_t v = (W4Type<T>::kMagic & 0xffffu) | (z & 15u);
+        if (kHalf) v = (uint32_t)__half_as_ushort(__hsub(__ushort_as_half((uint16_t)v), __ushort_as_half(0x6400)));
+        return s16 | v << 16;
+    };
+    const bool two = ((p.groups & 1) | (reinterpret_cast<uintptr_t>(p.scales) & 3) | (reinterpret_cast<uintptr_t>(p.zeros) & 1)) == 0;
     auto stage_scales = [&](int kb0) {
         const int g0 = kb0 * G, n = p.groups - g0 < kW4ChunkBlocks * G ? p.groups - g0 : kW4ChunkBlocks * G;
         const int want = (n + G - 1) / G * G;                      // groups behind K: every activation there is zero, any scale will do
         constexpr int RW = (ROWS + W - 1) / W;
+        if (G > 1 && two) {                                        // (a path more in groups of 128 cost 4096 x 4096 on one row 0.2 us of 5.2)
+            for (int i = lane * 2; i < want; i += 64) {
+                const int c = i < n ? i : n - 2;
+                uint32_t sv[RW], zv[RW];
+#pragma unroll
+                for (int q = 0; q < RW; q++) {
+                    const int r = warp + q * W;
+                    const long long at = (base_row + (row0 + r < p.M ? r : p.M - 1 - row0)) * p.groups + g0 + c;
+                    sv[q] = __ldg(reinterpret_cast<const uint32_t*>(p.scales + at));
+                    zv[q] = p.zeros ? (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(p.zeros + at)) : 0x0808u;
+                }
+#pragma unroll
+                for (int q = 0; q < RW; q++)
+                    if (warp + q * W < ROWS)
+                        *reinterpret_cast<uint2*>(&s_sz[(warp + q * W) * PITCH + i]) = make_uint2(pack_sz(sv[q] & 0xffffu, zv[q]), pack_sz(sv[q] >> 16, zv[q] >> 8));
+            }
+            return;
+        }
         for (int i = lane; i < want; i += 32) {
             const int c = i < n ? i : n - 1;
             uint32_t sv[RW], zv[RW];
@@ -180,13 +206,11 @@ __global__ void __launch_bounds__(W * 32, w4_resident_warps<T>(H) / W) w4_stream
                 const int r = warp + q * W;
                 const long long at = (base_row + (row0 + r < p.M ? r : p.M - 1 - row0)) * p.groups + g0 + c;
                 sv[q] = __ldg(p.scales + at);
-                zv[q] = p.zeros ? __ldg(p.zeros + at) & 15u : 8u;
+                zv[q] = p.zeros ? (uint32_t)__ldg(p.zeros + at) : 8u;
             }
 #pragma unroll
-            for (int q = 0; q < RW; q++) {
-                const float zf = (float)zv[q] + (kHalf ? 0.f : W4Type<T>::kMagicValue);
-                if (warp + q * W < ROWS) s_sz[(warp + q * W) * PITCH + i] = sv[q] | (uint32_t)W4Type<T>::from_float(zf) << 16;
-            }
+            for (int q = 0; q < RW; q++)
+                if (warp + q * W < ROWS) s_sz[(warp + q * W) * PITCH + i] = pack_sz(sv[q], zv[q]);
         }
     };
 
