@@ -130,3 +130,26 @@ def test_combine_unused_rows_and_refusals(L):
                  lambda: L.moe_combine(y.clone().requires_grad_(True), slots, weights)):
         with pytest.raises(RuntimeError):
             call()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("M", [1, 7, 8, 9, 15, 16, 20, 22, 41, 1025])
+def test_combine_any_alignment(L, M, dtype):
+    """Rows on every even address, in and out (the result's rows follow one another, M values apart): the sums are those of
+    16-byte aligned rows, bit for bit."""
+    g = torch.Generator(device="cuda").manual_seed(M)
+    T, k = 13, 5
+    y = torch.randn(T * k, M, generator=g, device="cuda").to(DT[dtype])
+    slots = torch.randperm(T * k, generator=g, device="cuda").int().view(T, k)
+    weights = torch.rand(T, k, generator=g, device="cuda")
+    room = torch.zeros(T * k, (M + 7) // 8 * 8, dtype=DT[dtype], device="cuda")
+    room[:, :M] = y
+    want = L.moe_combine(room, slots, weights)[:, :M]
+    ref, mag = W.combine(y, slots, weights)
+    assert bool(((want.double() - ref).abs() <= W.half_step(DT[dtype]) * ref.abs() + 2.0 ** -25 + k * 2.0 ** -24 * mag).all())
+    for pitch in (M, M + 1, M + 2, M + 4, M + 8):
+        for start in (0, 1, 2, 4):
+            buf = torch.full((T * k * pitch + start + 8,), float("nan"), dtype=DT[dtype], device="cuda")
+            src = buf[start:start + T * k * pitch].view(T * k, pitch)[:, :M]
+            src.copy_(y)
+            assert torch.equal(L.moe_combine(src, slots, weights), want)
