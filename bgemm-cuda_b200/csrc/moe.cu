@@ -375,62 +375,6 @@ int launch_moe_route(cudaStream_t stream, const void* logits, int dtype, long lo
     return route_dtype<BGEMM_DT_F32>(stream, logits, T, E, ld, top_k, renormalize, weights, experts, offsets, rows, slots, ws);
 }
 
-// Eight 16-bit values that start on an even address, loaded as what the address allows: one, two or four pieces, or, on an odd
-// 4-byte boundary, a half word, three words and a half word. `v` is put in order by octet_values, so that several are on their way at once.
-struct Octet {
-    uint32_t v[5];
-    bool odd;
-};
-__device__ __forceinline__ void load_octet(Octet& o, const uint16_t* src, int valid) {
-    const uint32_t low = (uint32_t)reinterpret_cast<uintptr_t>(src) & 15u;
-    o.odd = false;
-    if (valid < 8) {
-        o.v[0] = o.v[1] = o.v[2] = o.v[3] = 0u;
-#pragma unroll
-        for (int c = 0; c < 7; c++)
-            if (c < valid) o.v[c >> 1] |= (uint32_t)__ldg(src + c) << (16 * (c & 1));
-    } else if (low == 0) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(src));
-        o.v[0] = a.x; o.v[1] = a.y; o.v[2] = a.z; o.v[3] = a.w;
-    } else if (low == 8) {
-        const uint2 a = __ldg(reinterpret_cast<const uint2*>(src)), b = __ldg(reinterpret_cast<const uint2*>(src) + 1);
-        o.v[0] = a.x; o.v[1] = a.y; o.v[2] = b.x; o.v[3] = b.y;
-    } else if (low % 4 == 0) {
-#pragma unroll
-        for (int c = 0; c < 4; c++) o.v[c] = __ldg(reinterpret_cast<const uint32_t*>(src) + c);
-    } else {
-        o.odd = true;
-        o.v[0] = __ldg(src);
-#pragma unroll
-        for (int c = 0; c < 3; c++) o.v[1 + c] = __ldg(reinterpret_cast<const uint32_t*>(src + 1) + c);
-        o.v[4] = __ldg(src + 7);
-    }
-}
-__device__ __forceinline__ void octet_values(const Octet& o, uint32_t (&e)[4]) {
-    e[0] = o.odd ? o.v[0] | o.v[1] << 16 : o.v[0];
-    e[1] = o.odd ? __funnelshift_r(o.v[1], o.v[2], 16) : o.v[1];
-    e[2] = o.odd ? __funnelshift_r(o.v[2], o.v[3], 16) : o.v[2];
-    e[3] = o.odd ? __funnelshift_r(o.v[3], o.v[4], 16) : o.v[3];
-}
-__device__ __forceinline__ void store_octet(uint16_t* dst, int valid, const uint32_t (&e)[4]) {
-    const uint32_t low = (uint32_t)reinterpret_cast<uintptr_t>(dst) & 15u;
-    if (valid < 8) {
-#pragma unroll
-        for (int c = 0; c < 7; c++)
-            if (c < valid) dst[c] = (uint16_t)(e[c >> 1] >> (16 * (c & 1)));
-    } else if (low == 0) {
-        *reinterpret_cast<uint4*>(dst) = make_uint4(e[0], e[1], e[2], e[3]);
-    } else if (low % 4 == 0) {
-#pragma unroll
-        for (int c = 0; c < 4; c++) reinterpret_cast<uint32_t*>(dst)[c] = e[c];
-    } else {
-        dst[0] = (uint16_t)e[0];
-#pragma unroll
-        for (int c = 0; c < 3; c++) reinterpret_cast<uint32_t*>(dst + 1)[c] = __funnelshift_r(e[c], e[c + 1], 16);
-        dst[7] = (uint16_t)(e[3] >> 16);
-    }
-}
-
 // out[t, m] = sum_j weights[t, j] * y[slots[t, j], m], j in ascending order in 32 bits, rounded once; a slot outside
 // [0, slots_total) adds nothing. A thread owns 8 columns of a token, the loads of four slots in flight. ALIGNED: whole octets on 16-byte
 // boundaries everywhere (8000 x 4104, 4 slots: 55.3 us; 8000 x 4097 by octets of any alignment 78.5, value by value 107).

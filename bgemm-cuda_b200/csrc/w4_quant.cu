@@ -8,7 +8,7 @@
 // Both kernels are bound by memory: 2 (4) bytes in and half a byte out per weight, or the reverse. A lane owns 8 consecutive
 // columns -- one 16-byte load and one word of codes --, sixteen lanes a storage block; the group's extremes are exchanged with
 // 2 to 4 shuffles. A warp takes 1024 columns of a row at a time, four loads of a lane on their way (one at a time, with a 64-bit
-// division for its place, took 450 us for both kernels on 28672 x 8192 bf16, groups of 64; now 142 + 94, 182 at the copy bandwidth; the way there is bound by its arithmetic, the way back by memory).
+// division for its place, took 450 us for both kernels on 28672 x 8192 bf16, groups of 64; now 130 + 94, 182 at the copy bandwidth; the way there is bound by its arithmetic, the way back by memory).
 #include <cuda_runtime.h>
 
 #include "internal.h"
@@ -108,21 +108,20 @@ __device__ __forceinline__ float pick8(const float (&v)[8], int i) {
     return f;
 }
 
-// rint(w / s), inv = 1 / s to a place or two. The quotient is corrected once by its exact remainder (P. Markstein, "Computation of
-// elementary functions on the IBM RISC System/6000 processor", 1990), after which it is off by less than 2^-44 before its own
-// rounding: where w / s is exactly a half it is that half, and two numbers of 11 bits that do not divide to a half stay 2^-22
-// away from one, so the whole number is the division's own. (A test of |w - r s| against s / 2 that sends only doubtful octets to
-// a division took 259 us on 28672 x 8192 bf16: two in five warps held a tie.)
-__device__ __forceinline__ float quotient_rint(float w, float s, float inv) {
-    const float magic = 12582912.f;                                // 1.5 * 2^23: adding it rounds to a whole number, ties to even
-    float t = __fmul_rn(w, inv);
-    t = __fmaf_rn(__fmaf_rn(-t, s, w), inv, t);
-    return __fsub_rn(__fadd_rn(t, magic), magic);
-}
+// w / s where inv + low = 1 / s: inv to a place or two, low its remainder (1 - s inv) inv -- one step of P. Markstein, "Computation of
+// elementary functions on the IBM RISC System/6000 processor", 1990, taken once for eight columns. The sum of the products is off by
+// less than 2^-43 before its own rounding: where w / s is exactly a half it is that half, and a quotient of a number of 24 bits by one of 11 that
+// is no midpoint of two floats stays 2^-36 away from one, so this is the division's own result. (A test of |w - r s| against s / 2
+// that sends only doubtful octets to a division took 259 us on 28672 x 8192 bf16: two in five warps held a tie. Correcting each quotient
+// by its own remainder, and packing the codes as floats, 140; now 130.)
+__device__ __forceinline__ float quotient(float w, float inv, float low) { return __fmaf_rn(w, inv, __fmul_rn(w, low)); }
+// 1.5 * 2^23: adding it rounds to a whole number, ties to even, whose two's complement is then in the low bits
+constexpr float kRound = 12582912.f;
+constexpr uint32_t kRoundBits = 0x4B400000u;
 
-// LG: log2 of the lanes (8 columns each) of a group. SYM: symmetric codes.
+// LG: log2 of the lanes (8 columns each) of a group. SYM: symmetric codes. Four CTAs an SM (67 registers, three CTAs: 181 us on 28672 x 8192 bf16 with zero points in groups of 128, 159 with four); fp32 has three.
 template <int DT, typename S, int LG, bool SYM>
-__global__ void __launch_bounds__(256) w4_quantize_kernel(const void* __restrict__ src, long long M, int K, long long ld, uint32_t* __restrict__ plane,
+__global__ void __launch_bounds__(256, DT == BGEMM_DT_F32 ? 3 : 4) w4_quantize_kernel(const void* __restrict__ src, long long M, int K, long long ld, uint32_t* __restrict__ plane,
                                                           uint16_t* __restrict__ scales, uint8_t* __restrict__ zeros, long long batch_stride, int piece) {
     grid_dependency_wait();
     const int chunks = (K + 127) / 128 * 16;                       // 8-column chunks per row, whole blocks
@@ -136,7 +135,6 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const void* __restrict
     plane += batch * M * chunks;
     scales += batch * M * groups;
     if (!SYM) zeros += batch * M * groups;
-    constexpr float magic = 12582912.f;
     for (long long st = (long long)blockIdx.x * 8 + warp; st < steps; st += nwarps) {
         // M <= 2^24 rows of at most 2^14 units
         const long long m = units == 1 ? st : (st < (1LL << 32) ? (long long)((unsigned)st / units) : st / units);
@@ -166,37 +164,40 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const void* __restrict
             float z = SYM ? 8.f : 0.f;
             uint32_t word;
             if (s > 0.f) {
-                const float inv = __fdividef(1.f, s);
-                float v[8], r[8], zr = 0.f;
+                const float inv = __fdividef(1.f, s), low = __fmul_rn(__fmaf_rn(-s, inv, 1.f), inv);
+                float v[8], zr = 0.f, most = 16.f;                        // most: the largest code, before its bound
+                uint32_t r[8];                                     // kRoundBits + rint(w / s)
                 floats8<DT>(raw[q], v);
-                if (s >= 1.2e-38f && s <= 4.0e37f) {
+                if (s >= 1.2e-38f && s <= 1.0e30f) {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) r[i] = quotient_rint(v[i], s, inv);
-                    if (!SYM) zr = quotient_rint(ext.x, s, inv);
-                } else {                                           // 1 / s is not a normal number
+                    for (int i = 0; i < 8; i++) r[i] = __float_as_uint(__fadd_rn(quotient(v[i], inv, low), kRound));
+                    if (!SYM) {
+                        zr = __fsub_rn(__fadd_rn(quotient(ext.x, inv, low), kRound), kRound);
+                        most = zr + __fsub_rn(__fadd_rn(quotient(ext.y, inv, low), kRound), kRound);
+                    }
+                } else {                                           // 1 / s or its remainder is not a normal number
 #pragma unroll 1
                     for (int i = 0; i < 9; i++) {
                         const float w = i == 8 ? ext.x : pick8(v, i), whole_number = rintf(__fdiv_rn(w, s));
                         if (i == 8 && !SYM) zr = whole_number;
+                        const uint32_t bits = __float_as_uint(__fadd_rn(whole_number, kRound));
 #pragma unroll
                         for (int j = 0; j < 8; j++)
-                            if (j == i) r[j] = whole_number;
+                            if (j == i) r[j] = bits;
                     }
                 }
                 if (!SYM) z = fminf(zr, 15.f);
+                const uint32_t zi = SYM ? 8u : __float_as_uint(__fadd_rn(z, kRound)) - kRoundBits;
                 // q = clamp(r + z, 0, 15). Below, the clamp is void (r(lowest) = -zr, symmetric r >= -7) unless s itself was rounded
-                // far, as a subnormal number, or z was cut; above, both roundings can add up to 16.
-                const float top = 15.f - z;
-                if (s < 6.2e-5f || zr > 15.f) {
+                // far, as a subnormal number, or z was cut; above, both roundings can add up to 16 (one group in sixty).
+                if (s < 6.2e-5f || (!SYM && (zr > 15.f || most > 15.f))) {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) r[i] = fminf(fmaxf(r[i], -z), top);
+                    for (int i = 0; i < 8; i++) r[i] = min(max(r[i], kRoundBits - zi), kRoundBits + 15u - zi);
                 }
-                // the nibbles of either half of the word are added up as one number below 2^16
-                float half[2];
-                half[0] = half[1] = magic + z * 4369.f;
+                // sum of q 16^nibble, modulo 2^32: what kRoundBits and z add is taken off once
+                word = (zi - kRoundBits) * 0x11111111u;
 #pragma unroll
-                for (int i = 0; i < 8; i++) half[i & 1] = __fmaf_rn(SYM ? r[i] : fminf(r[i], top), (float)(1 << (4 * (i >> 1))), half[i & 1]);
-                word = __byte_perm(__float_as_uint(half[0]), __float_as_uint(half[1]), 0x5410);
+                for (int i = 0; i < 8; i++) word += r[i] << (4 * ((i & 1) * 4 + (i >> 1)));
             } else {
                 word = SYM ? 0x88888888u : 0u;
             }
@@ -210,10 +211,10 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const void* __restrict
     }
 }
 
-template <typename T>
+// ALIGNED: every octet of the result lies on a 16-byte boundary (others: 4096 x 4097 15 us; value by value 44).
+template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256) w4_dequantize_kernel(const uint32_t* __restrict__ plane, long long M, int K, int lanes_log2,
-                                                            const uint16_t* __restrict__ scales, const uint8_t* __restrict__ zeros, uint16_t* __restrict__ out,
-                                                            int piece) {
+                                                            const uint16_t* __restrict__ scales, const uint8_t* __restrict__ zeros, uint16_t* __restrict__ out) {
     grid_dependency_wait();
     const int chunks = (K + 127) / 128 * 16, used = (K + 7) / 8;
     const unsigned units = (unsigned)(chunks + kQUnit - 1) / kQUnit;
@@ -246,19 +247,8 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(const uint32_t* __re
 #pragma unroll
             for (int p = 0; p < 4; p++) v[p] = w4_pair<T>(word[q] >> (4 * p), mz, s2, magic);
             uint16_t* dst = out + m * (long long)K + k0;
-            if (k0 + 8 <= K && piece == 16) {
-                __stcs(reinterpret_cast<uint4*>(dst), make_uint4(v[0], v[1], v[2], v[3]));
-            } else if (k0 + 8 <= K && piece == 8) {
-                __stcs(reinterpret_cast<uint2*>(dst), make_uint2(v[0], v[1]));
-                __stcs(reinterpret_cast<uint2*>(dst) + 1, make_uint2(v[2], v[3]));
-            } else if (k0 + 8 <= K && piece == 4) {
-#pragma unroll
-                for (int j = 0; j < 4; j++) __stcs(reinterpret_cast<uint32_t*>(dst) + j, v[j]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    if (k0 + j < K) dst[j] = (uint16_t)(v[j >> 1] >> (16 * (j & 1)));
-            }
+            if (ALIGNED) __stcs(reinterpret_cast<uint4*>(dst), make_uint4(v[0], v[1], v[2], v[3]));
+            else store_octet(dst, K - k0, v);
         }
     }
 }
@@ -310,11 +300,12 @@ int launch_w4_quantize(cudaStream_t stream, const void* src, int dtype, long lon
 
 int launch_w4_dequantize(cudaStream_t stream, const void* plane, long long M, long long K, int group, const void* scales, const void* zeros,
                          int dtype, void* out) {
-    const int piece = widest_piece(reinterpret_cast<uintptr_t>(out) | (uintptr_t)(M > 1 ? K * 2 : 0));
+    const bool aligned = reinterpret_cast<uintptr_t>(out) % 16 == 0 && K % 8 == 0;
     const dim3 grid(quant_blocks(M, K));
-    const auto kernel = dtype == BGEMM_DT_F16 ? w4_dequantize_kernel<__half> : w4_dequantize_kernel<__nv_bfloat16>;
+    const auto kernel = dtype == BGEMM_DT_F16 ? (aligned ? w4_dequantize_kernel<__half, true> : w4_dequantize_kernel<__half, false>)
+                                              : (aligned ? w4_dequantize_kernel<__nv_bfloat16, true> : w4_dequantize_kernel<__nv_bfloat16, false>);
     const cudaError_t e = launch_pdl(kernel, grid, dim3(256), stream, static_cast<const uint32_t*>(plane), M, (int)K, lanes_log2_of(group),
-                                     static_cast<const uint16_t*>(scales), static_cast<const uint8_t*>(zeros), static_cast<uint16_t*>(out), piece);
+                                     static_cast<const uint16_t*>(scales), static_cast<const uint8_t*>(zeros), static_cast<uint16_t*>(out));
     count_launch();
     return (int)(e != cudaSuccess ? e : cudaGetLastError());
 }
