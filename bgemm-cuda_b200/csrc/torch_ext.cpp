@@ -403,10 +403,11 @@ torch::Tensor w4_dequantize(torch::Tensor plane, torch::Tensor scales, c10::opti
     return out;
 }
 
-// The tensor-core path loads x by TMA, whose rows start on 16-byte boundaries: a copy with such a pitch where x has another one
-// and there are more rows than two passes of the other kernel take.
-torch::Tensor rows_on_16_bytes(const torch::Tensor& x, int64_t products) {
-    if (products <= 16 || (reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && (x.size(0) == 1 || x.stride(0) % 8 == 0))) return x;
+// The tensor-core path loads x by TMA, whose rows start on 16-byte boundaries, and the other kernel is slowed down by rows that do not
+// (28672 x 8190 on 8 rows 51 us, 36 with the copy): a copy with such a pitch where x has another one, and there are more rows than two
+// passes take or so many codes that the call lasts longer than the copy's ~6 us on the host (4096 x 4095 on 8 rows: 10 us as it is).
+torch::Tensor rows_on_16_bytes(const torch::Tensor& x, int64_t products, double codes) {
+    if ((products <= 16 && (products == 1 || codes < 64e6)) || (reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && (x.size(0) == 1 || x.stride(0) % 8 == 0))) return x;
     const int64_t K = x.size(1);
     auto copy = torch::empty({x.size(0), (K + 7) / 8 * 8}, x.options()).narrow(1, 0, K);
     copy.copy_(x.detach());
@@ -425,7 +426,7 @@ torch::Tensor w4a16_linear_forward(torch::Tensor x, torch::Tensor plane, torch::
     if (x.stride(1) != 1 || (N > 1 && x.stride(0) < K)) x = x.contiguous();
     auto out = fresh({N, M}, x.scalar_type());
     if (out.numel() == 0) return out;
-    x = rows_on_16_bytes(x, N);
+    x = rows_on_16_bytes(x, N, (double)M * (double)K);
     const size_t need = bgemm_w4a16_workspace_bytes(1, M, K, N);
     torch::Tensor ws;
     if (need) ws = fresh({(int64_t)need}, at::kByte);
@@ -467,7 +468,7 @@ torch::Tensor w4a16_grouped_forward(torch::Tensor x, torch::Tensor plane, torch:
         TORCH_CHECK(out.numel() == 0, where, ": x has no rows");
         return out;
     }
-    x = rows_on_16_bytes(x, slots);
+    x = rows_on_16_bytes(x, slots, (double)M * (double)K * (double)std::min(slots, E));
     const size_t need = bgemm_w4a16_workspace_bytes(E, M, K, slots);
     torch::Tensor ws;
     if (need) ws = fresh({(int64_t)need}, at::kByte);
