@@ -79,15 +79,15 @@ template <int GW>
 __host__ __device__ constexpr int w4_pitch() { return kW4ChunkBlocks * (4 / GW) + 4; }                  // 4 mod 32, 16-byte rows: the eight rows of a read meet eight banks
 
 // Warps an SM is meant to hold. Registers spill at what 24 leave each with five octets of fp16 rows (28672 x 8192 on 8 rows in
-// groups of 64: 47 us, 40 with 20 warps; bf16 31.1 and 32.3) and with four scale groups a block (in groups of 32: 58 us, 49 with 16; fp16
-// 73 and 56).
+// groups of 64: 47 us, 40 with 20 warps; bf16 31.1 and 32.3), with four scale groups a block (in groups of 32: 58 us, 49 with 16; fp16
+// 73 and 56), and with two where eight warps share K (8192 x 8192 on 4 rows 14.6 us, 12.4 with 16, on two tiles an SM anyway).
 template <typename T>
-__host__ __device__ constexpr int w4_resident_warps(int H, int GW) { return GW == 1 && H > 2 ? 16 : (H > 4 && W4Type<T>::kMagicValue == 1024.f ? 20 : 24); }
+__host__ __device__ constexpr int w4_resident_warps(int W, int H, int GW) { return H > 2 && (GW == 1 || (GW == 2 && W == 8)) ? 16 : (H > 4 && W4Type<T>::kMagicValue == 1024.f ? 20 : 24); }
 
 // W: warps of a CTA (K is divided among them), H: its weight rows in octets (two make a 16-row product, an odd one a product
 // whose other half is zero), GW: 32-column words per scale group (1, 2, 4).
 template <typename T, int W, int H, int GW>
-__global__ void __launch_bounds__(W * 32, w4_resident_warps<T>(H, GW) / W) w4_stream_kernel(const W4Gemm p) {
+__global__ void __launch_bounds__(W * 32, w4_resident_warps<T>(W, H, GW) / W) w4_stream_kernel(const W4Gemm p) {
     constexpr bool kHalf = W4Type<T>::kMagicValue == 1024.f;
     constexpr int MT = (H + 1) / 2, G = 4 / GW, PITCH = w4_pitch<GW>(), ROWS = H * 8, STEP_BYTES = ROWS * kW4BlockBytes;
     // Per warp a ring of blocks that every lane fills and reads back itself (no barrier anywhere near it), then the scales

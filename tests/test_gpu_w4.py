@@ -1,5 +1,7 @@
 """GPU tests of the 4-bit weight operators against the plain 64-bit implementations of oracle/w4_oracle.py. Tolerances are
 w4_oracle.linear_tolerance (roundings counted one by one) unless a test says exact."""
+import os
+
 import pytest
 import torch
 
@@ -332,9 +334,10 @@ def test_one_expert_with_an_index_is_the_dense_product(L):
     plane, scales, zeros = matrix((1,), M, K, group, torch.bfloat16, True, g)
     x = torch.randn(200, K, generator=g, device="cuda").bfloat16()
     rows = torch.randint(0, 200, (n,), generator=g, device="cuda", dtype=torch.int32)
-    assert B.lib.bgemm_w4a16_workspace_bytes(1, M, K, n) >= n * K * 2
     got = L.w4a16_grouped_forward(x, plane, scales, zeros, ragged([n]), rows, group)
-    assert torch.equal(got, L.w4a16_linear_forward(x[rows.long()], plane[0], scales[0], zeros[0], group))
+    if os.environ.get("BGEMM_W4_TENSOR") != "0":                            # (the other kernel wants no workspace, and adds in another order)
+        assert B.lib.bgemm_w4a16_workspace_bytes(1, M, K, n) >= n * K * 2
+        assert torch.equal(got, L.w4a16_linear_forward(x[rows.long()], plane[0], scales[0], zeros[0], group))
     check_linear(got, x[rows.long()], plane[0], scales[0], zeros[0], K, group)
 
 
