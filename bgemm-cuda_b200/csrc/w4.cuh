@@ -139,6 +139,9 @@ __device__ __forceinline__ void store_octet(uint16_t* dst, int valid, const uint
             if (c < valid) dst[c] = (uint16_t)(e[c >> 1] >> (16 * (c & 1)));
     } else if (low == 0) {
         *reinterpret_cast<uint4*>(dst) = make_uint4(e[0], e[1], e[2], e[3]);
+    } else if (low == 8) {
+        reinterpret_cast<uint2*>(dst)[0] = make_uint2(e[0], e[1]);
+        reinterpret_cast<uint2*>(dst)[1] = make_uint2(e[2], e[3]);
     } else if (low % 4 == 0) {
 #pragma unroll
         for (int c = 0; c < 4; c++) reinterpret_cast<uint32_t*>(dst)[c] = e[c];
