@@ -356,3 +356,22 @@ def test_a_gradient_is_refused_wherever_it_is_asked(L):
     with torch.no_grad():
         want = L.w4a16_grouped_forward(x, plane, scales, zeros, off, None, 64)
         assert torch.equal(L.w4a16_grouped_forward(x, plane, learnt, zeros, off, None, 64, out), want)
+
+
+@pytest.mark.parametrize("M", [256, 300, 257])
+@pytest.mark.parametrize("pitch,start", [(320, 0), (320, 1), (320, 2), (320, 4), (324, 0), (322, 2), (321, 0), (321, 3)])
+def test_results_at_any_alignment(L, M, pitch, start):
+    """Many rows (tensor cores) into a buffer with that pitch from that element: the values of a plain call, and nothing else written."""
+    g = gen(M + pitch + start)
+    K, n, group, E = 1024, 700, 64, 3
+    plane, scales, zeros = matrix((E,), M, K, group, torch.bfloat16, True, g)
+    x = torch.randn(n, K, generator=g, device="cuda").bfloat16()
+    off = ragged([100, 0, 500])
+    want = L.w4a16_grouped_forward(x, plane, scales, zeros, off, None, group)
+    check_linear(want[:100], x[:100], plane[0], scales[0], zeros[0], K, group)
+    check_linear(want[100:600], x[100:600], plane[2], scales[2], zeros[2], K, group)
+    buf = torch.full((n * pitch + start,), 7.0, dtype=torch.bfloat16, device="cuda")
+    rows = buf[start:].view(n, pitch)
+    L.w4a16_grouped_forward(x, plane, scales, zeros, off, None, group, rows[:, :M])
+    assert torch.equal(rows[:600, :M], want[:600])
+    assert bool((rows[600:] == 7).all()) and bool((rows[:, M:] == 7).all()) and bool((buf[:start] == 7).all())
