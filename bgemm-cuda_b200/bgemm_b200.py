@@ -59,6 +59,10 @@ lib.bgemm_gemm_workspace_bytes.restype = _sz
 lib.bgemm_gemm_workspace_bytes.argtypes = [_i64, _i64, _i64, _int, _i64]
 lib.bgemm_debug_set_pair_kernel.restype = None
 lib.bgemm_debug_set_pair_kernel.argtypes = [_int]
+lib.bgemm_debug_set_w4_kernel.restype = None
+lib.bgemm_debug_set_w4_kernel.argtypes = [_int]
+lib.bgemm_debug_w4_calls.restype = ctypes.c_uint64
+lib.bgemm_debug_w4_calls.argtypes = [_int]
 lib.bgemm_gemm_balance_workspace_bytes.restype = _sz
 lib.bgemm_gemm_balance_workspace_bytes.argtypes = [_i64, _i64, _i64, _int, _i64]
 lib.bgemm_gemm_auto_split_k.argtypes = [_i64, _i64, _i64, _i64]

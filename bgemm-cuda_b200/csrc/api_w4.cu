@@ -1,4 +1,5 @@
 // extern "C" surface of the 4-bit weight products and the expert routing (include/bgemm_b200.h): argument checks and launches.
+#include <atomic>
 #include <cstdlib>
 
 #include "internal.h"
@@ -14,6 +15,19 @@ constexpr int kMaxExperts = 1024, kMaxTopK = 32;
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 bool group_ok(int g) { return g == 32 || g == 64 || g == 128; }
 bool is16(int d) { return d == BGEMM_DT_F16 || d == BGEMM_DT_BF16; }
+
+// bgemm_debug_set_w4_kernel: 0 streaming, 1 tensor cores, -1 the rule below; -2 not set, where BGEMM_W4_TENSOR (read once) says the same.
+std::atomic<int> g_w4_kernel{-2};
+std::atomic<uint64_t> g_w4_calls[2];             // products that each kernel has taken: streaming, tensor cores
+
+int forced_kernel() {
+    static const int env = [] {
+        const char* e = std::getenv("BGEMM_W4_TENSOR");
+        return e ? std::atoi(e) : -1;
+    }();
+    const int m = g_w4_kernel.load(std::memory_order_relaxed);
+    return m == -2 ? env : m;
+}
 
 int check_matrix(int64_t M, int64_t K, int group) {
     if (!group_ok(group)) return BGEMM_ERR_ENUM;
@@ -55,13 +69,9 @@ W4Gemm problem(const void* plane, int E, int64_t M, int64_t K, int group, const 
 // rows each 72 / 98, on 12 129 / 99; 8 of them on 93 rows 24 / 19. So: by the bytes of all passes, a short row counting as
 // 1536 columns (a CTA's own start and end; 18 experts of 11964 x 128 on 160 rows: 61 / 33). Rows of x off 16-byte
 // boundaries cannot be loaded by TMA and stay on the former.
-// Tuning override (read once, unset in normal use): BGEMM_W4_TENSOR = 0 never, 1 whenever the rows of x allow it.
 bool on_tensor_cores(const W4Gemm& p) {
     if (!p.x_vec) return false;
-    static const int forced = [] {
-        const char* e = std::getenv("BGEMM_W4_TENSOR");
-        return e ? std::atoi(e) : -1;
-    }();
+    const int forced = forced_kernel();
     if (forced >= 0) return forced != 0;
     const double matrix = (double)p.M * (p.K > 1536 ? (double)p.K : 1536.0) / 2;
     if (!p.offsets) {
@@ -74,7 +84,9 @@ bool on_tensor_cores(const W4Gemm& p) {
 }
 
 int run(cudaStream_t stream, const W4Gemm& p, int dtype, void* workspace, size_t workspace_bytes) {
-    if (!on_tensor_cores(p)) return launch_w4_stream(stream, p, dtype);
+    const bool tensor = on_tensor_cores(p);
+    g_w4_calls[tensor].fetch_add(1, std::memory_order_relaxed);
+    if (!tensor) return launch_w4_stream(stream, p, dtype);
     const size_t need = w4_umma_workspace(p);
     return launch_w4_umma(stream, p, dtype, need && workspace && workspace_bytes >= need ? workspace : nullptr);
 }
@@ -139,6 +151,9 @@ int bgemm_w4a16_grouped_gemm(void* stream, const void* plane, int64_t E, int64_t
     p.rows = rows;
     return run((cudaStream_t)stream, p, dtype, workspace, workspace_bytes);
 }
+
+void bgemm_debug_set_w4_kernel(int mode) { g_w4_kernel.store(mode < -1 || mode > 1 ? -2 : mode, std::memory_order_relaxed); }
+uint64_t bgemm_debug_w4_calls(int tensor) { return g_w4_calls[tensor ? 1 : 0].load(std::memory_order_relaxed); }
 
 size_t bgemm_moe_route_workspace_bytes(int64_t T, int64_t E) {
     if (T < 1 || E < 1 || E > kMaxExperts || T > kMaxSlots) return 0;

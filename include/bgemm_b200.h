@@ -414,6 +414,13 @@ void bgemm_debug_set_wait_test(int64_t wait_budget_clocks, int skip_kblock);
  * environment variable sets the same at load time). Process-wide; results never depend on it.             */
 void bgemm_debug_set_pair_kernel(int mode);
 
+/* The same for the 4-bit products (bgemm_w4a16_gemm, bgemm_w4a16_grouped_gemm and their workspace query): 0 = every call on
+ * the streaming kernel, 1 = every call whose rows of x start on 16-byte boundaries on the tensor cores, -1 = the library's own rule (the
+ * default; the BGEMM_W4_TENSOR environment variable sets the same at load time). Process-wide. bgemm_debug_w4_calls returns how
+ * many products the streaming kernel (tensor = 0) or the tensor-core kernel (1) has taken in this process.          */
+void bgemm_debug_set_w4_kernel(int mode);
+uint64_t bgemm_debug_w4_calls(int tensor);
+
 #ifdef __cplusplus
 }
 #endif

@@ -103,6 +103,35 @@ def linear_tolerance(x, y, plane, scales, zeros, K, group) -> torch.Tensor:
     return u * y.abs() + tiny + u * (ax @ weights.t()) + tiny * ax.sum(1, keepdim=True) + steps * 2.0 ** -23 * (ax @ parts.t())
 
 
+def rounded(plane, scales, zeros, K, group) -> torch.Tensor:
+    """values(..) as the tensor-core kernel multiplies them: each rounded once to the scales' type (in 64 bits)."""
+    return values(plane, scales, zeros, K, group).to(scales.dtype).double()
+
+
+def linear_bound(x, y, plane, scales, zeros, K, group, tensor) -> torch.Tensor:
+    """How far one kernel's result may be from `y`, element by element. tensor: the tensor-core kernel, y = linear(x, rounded(..));
+    otherwise the streaming kernel, which rounds no weight, y = linear(x, values(..)). Both:
+      * one rounding of the result: u |y| (u = half a step of the 16-bit type, 2^-25 below the normal numbers of fp16);
+      * one product of 16 columns adds 16 parts to a sum, each addition off by at most 2^-23 of it (the tensor cores may truncate):
+        17 * 2^-23 a product with its start.
+    Tensor cores: ceil(K / 16) such products on parts |w x|, and up to 8 partial sums added up, 2^-24 each.
+    Streaming: group / 16 products (and 4 roundings where the group's sums meet scale and zero point) on parts (q + z) s |x|,
+    (q + z + 256) s |x| for bf16, whose codes are summed as 128 + q; the groups and the sums of up to 12 warps meet by additions of
+    2^-24 of sums no larger than sum |w x|."""
+    u = half_step(x.dtype)
+    tiny = 2.0 ** -25 if x.dtype == torch.float16 else 0.0
+    ax = x.double().abs()
+    mag = ax @ (rounded if tensor else values)(plane, scales, zeros, K, group).abs().t()
+    if tensor:
+        sums = (17 * -(-K // 16) * 2.0 ** -23 + 8 * 2.0 ** -24) * mag
+    else:
+        q = unpack(plane, K).double()
+        z = 8.0 if zeros is None else spread((zeros & 15).double(), K, group)
+        parts = ax @ ((q + z + (256.0 if x.dtype == torch.bfloat16 else 0.0)) * spread(scales.double().abs(), K, group)).t()
+        sums = (17 * (group // 16) + 4) * 2.0 ** -23 * parts + (scales.shape[-1] + 16) * 2.0 ** -24 * mag
+    return u * (y.abs() + sums) + tiny + sums
+
+
 def route(logits, top_k, renormalize):
     """(weights float64 [T, k], experts, offsets, rows, slots) by plain loops over tokens."""
     T, E = logits.shape
