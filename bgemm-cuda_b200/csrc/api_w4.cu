@@ -66,21 +66,24 @@ W4Gemm problem(const void* plane, int E, int64_t M, int64_t K, int group, const 
 // any number of rows in one pass, but needs ~9 us to fill and drain and unpacks codes at less than half the memory's rate.
 // Measured (us, streaming / tensor cores): 4096 x 4096 on 16 rows 8 / 15, on 24 10 / 15, on 32 11 / 15; 11008 x 4096 on 16 rows
 // 14 / 17, on 24 20 / 17; 8192 x 8192 on 12 rows 19 / 22; 28672 x 8192 on 8 rows 31 / 50, on 16 57 / 50; 177 x 1720 on 709 rows 8 / 16; 64 experts of 2048 x 4096 on 8
-// rows each 72 / 98, on 12 129 / 99; 8 of them on 93 rows 24 / 19. So: by the bytes of all passes, a short row counting as
+// rows each 82 / 104, on 9 133 / 104; 8 of them on 93 rows 24 / 19. So: by the bytes of all passes, a short row counting as
 // 1536 columns (a CTA's own start and end; 18 experts of 11964 x 128 on 160 rows: 61 / 33). Rows of x off 16-byte
 // boundaries cannot be loaded by TMA and stay on the former.
+// One pass always streams, whatever the matrix: no weight is rounded on up to eight rows, or eight slots an expert. The counts of
+// more experts than one are on the device, so that is by their average, and an expert's last pass is not full: 0.4 of one more.
+// (Eight slots on average, unevenly: 64 x 2048 x 4096 107 / 115, 16 x 4096 x 4096 59 / 65, 64 x 1001 x 2056 51 / 47. All 768 slots of 128 experts
+// of 2048 x 2048 on one of them: 70 / 22.)
 bool on_tensor_cores(const W4Gemm& p) {
     if (!p.x_vec) return false;
     const int forced = forced_kernel();
     if (forced >= 0) return forced != 0;
     const double matrix = (double)p.M * (p.K > 1536 ? (double)p.K : 1536.0) / 2;
-    if (!p.offsets) {
+    if (!p.offsets || p.E == 1) {
         const long long passes = (p.slots + 7) / 8;
         return passes > 1 && passes * matrix > (passes == 2 ? 80e6 : 45e6);
     }
-    // the counts are on the device: on average an expert's last pass is not full
     const double experts = (double)(p.slots < p.E ? p.slots : p.E), rows = (double)p.slots / experts;
-    return rows > 6 && experts * (rows / 8 + 0.4) * matrix > 45e6;
+    return rows > 8 && experts * (rows / 8 + 0.4) * matrix > 45e6;
 }
 
 int run(cudaStream_t stream, const W4Gemm& p, int dtype, void* workspace, size_t workspace_bytes) {
@@ -124,7 +127,7 @@ size_t bgemm_w4a16_workspace_bytes(int64_t E, int64_t M, int64_t K, int64_t slot
     static const int32_t some = 0;
     p.E = (int)E; p.M = (int)M; p.K = (int)K; p.slots = slots; p.x_vec = 1;
     const size_t dense = E == 1 && on_tensor_cores(p) ? w4_umma_workspace(p) : 0;
-    p.offsets = &some;                            // only whether there are any counts here; one matrix may be called either way
+    p.offsets = &some;                            // only whether there are any; one matrix may be called either way, with an index too
     const size_t grouped = on_tensor_cores(p) ? w4_umma_workspace(p) : 0;
     return dense > grouped ? dense : grouped;
 }

@@ -347,9 +347,9 @@ int bgemm_w4_dequantize(void* stream, const void* plane, int64_t M, int64_t K, i
 
 /* y[n, m] = sum_k x[n, k] w[m, k]: x [N, K] (row pitch x_ld elements) and out [N, M] (row pitch out_ld) of `dtype`, which
  * is also the scales' type; sums in 32 bits, rounded once. Any N, M, K and alignment of x.
- * Few rows (up to 8 always, up to some dozens where the matrix is small; rows of x off 16-byte boundaries at any N, more
- * slowly) meet the weights as the exact products above. For more, each weight is first rounded to the 16-bit type, as
- * bgemm_w4_dequantize returns it: scales so small that (q - z) s is no normal fp16 number lose bits there.
+ * Two kernels, chosen by sizes alone. Up to 8 rows, all calls whose rows of x start off 16-byte boundaries, and more rows while
+ * ceil(N / 8) passes over the matrix stay small (M max(K, 1536) / 2 bytes each: 45 MB in all, 80 MB for two passes) meet the weights as the exact
+ * products above. For others each weight is first rounded once to the 16-bit type, as bgemm_w4_dequantize returns it.
  * bf16: |x| up to 1e34 (128 columns' sums of (128 + q) x are held in 32 bits before the zero point comes off).
  * out must not overlap x, the plane or the scales.
  * workspace: optional, bgemm_w4a16_workspace_bytes(1, M, K, N) bytes of any contents, 256-byte aligned: partial sums of
@@ -365,8 +365,10 @@ int bgemm_w4a16_gemm(void* stream, const void* plane, int64_t M, int64_t K, int 
  * [offsets[e], offsets[e + 1]) is multiplied with expert e's matrix: out[s] = W_e x[rows ? rows[s] : s]. `offsets` is a
  * device array int32 [E + 1], ascending from 0 to at most `slots`; experts may be empty; out rows behind offsets[E] are
  * not written. `rows` (device, int32 [slots], or NULL) names the row of x [x_rows, K] a slot reads; an index outside x
- * counts as a row of zeros. workspace as above, bgemm_w4a16_workspace_bytes(E, M, K, slots). The host never reads offsets
- * or rows; whatever they hold, no access leaves the buffers.                                                            */
+ * counts as a row of zeros. The choice of kernel goes by the slots of an expert on average, slots / min(slots, E): up to 8 always
+ * meet exact weights, more while all experts' passes together stay below 45 MB; E = 1 is the dense product's rule.
+ * workspace as above, bgemm_w4a16_workspace_bytes(E, M, K, slots). The host never reads offsets or rows; whatever they hold, no access
+ * leaves the buffers.                                                                                                   */
 int bgemm_w4a16_grouped_gemm(void* stream, const void* plane, int64_t E, int64_t M, int64_t K, int group, const void* scales,
                              const uint8_t* zeros, const void* x, int64_t x_rows, int64_t x_ld, int dtype, const int32_t* offsets,
                              const int32_t* rows, int64_t slots, void* out, int64_t out_ld, void* workspace,

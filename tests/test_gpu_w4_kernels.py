@@ -359,3 +359,48 @@ def test_both_bindings_and_the_layers(L, kernel, dtype):
         sl.copy_(ls[i])
         graph.replay()
         assert torch.equal(out, want[i])
+
+
+# ---- which kernel a call takes -----------------------------------------------------------------------------------------
+def calls():
+    import bgemm_b200 as B
+
+    return [B.lib.bgemm_debug_w4_calls(i) for i in (0, 1)]
+
+
+def telling(E, M, K, group, n, dtype):
+    """Two weights of a row, 15 s with a scale of many bits and 15, and activations 1 and -1 for them: 15 s - 15 where no weight is rounded
+    (a number of 4 bits); 15 s rounded to the type is another."""
+    s = 1 + (2.0 ** -10 if dtype == torch.float16 else 2.0 ** -7)
+    plane = torch.full((E, M, W.row_bytes(K)), 255, dtype=torch.uint8, device="cuda")
+    scales = torch.ones(E, M, -(-K // group), dtype=dtype, device="cuda")
+    scales[..., 0] = s
+    x = torch.zeros(n, K, dtype=dtype, device="cuda")
+    x[:, 0], x[:, group] = 1, -1
+    exact, off = 15 * s - 15, float(torch.tensor(15 * s).to(dtype)) - 15
+    assert exact != off
+    return plane, scales, torch.zeros(scales.shape, dtype=torch.uint8, device="cuda"), x, exact, off
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("E,M,K,per", [(1, 28672, 8192, 7), (1, 28672, 8192, 8), (64, 2048, 4096, 7), (64, 2048, 4096, 8)])
+def test_up_to_eight_slots_an_expert_meet_unrounded_weights(L, E, M, K, per, dtype):
+    n = E * per
+    plane, scales, zeros, x, exact, _ = telling(E, M, K, 128, n, DT[dtype])
+    before = calls()
+    got = L.w4a16_grouped_forward(x, plane, scales, zeros, ragged([per] * E), None, 128)
+    assert bool((got == exact).all())
+    assert bool((L.w4a16_linear_forward(x[:per], plane[0], scales[0], zeros[0], 128) == exact).all())
+    assert [b - a for a, b in zip(before, calls())] == [2, 0]
+
+
+@pytest.mark.parametrize("n", [8, 9, 16, 17, 40])
+@pytest.mark.parametrize("M,K", [(28672, 8192), (8192, 8192), (1024, 4096)])
+def test_one_expert_takes_the_kernel_of_the_dense_product(L, M, K, n):
+    plane, scales, zeros, x, exact, off = telling(1, M, K, 64, n, torch.bfloat16)
+    before = calls()
+    dense = L.w4a16_linear_forward(x, plane[0], scales[0], zeros[0], 64)
+    middle = calls()
+    assert torch.equal(L.w4a16_grouped_forward(x, plane, scales, zeros, ragged([n]), None, 64), dense)
+    assert [b - a for a, b in zip(before, middle)] == [b - a for a, b in zip(middle, calls())]
+    assert bool((dense == (exact if middle[0] > before[0] else off)).all())
