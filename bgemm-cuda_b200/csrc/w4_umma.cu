@@ -74,6 +74,7 @@ struct W4UmmaParams {
     long long wait_budget;
     int splits;
     int mpairs;                  // tiles of 256 weight rows
+    int test_skip_kblock;        // bgemm_debug_set_wait_test; -1: none
 };
 
 // kind::f16, both operands K-major, 32-bit accumulator, M = 256 over the pair.
@@ -341,6 +342,7 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
                 for (int i = u.kb0; i < u.kb1; i++, ring.step()) {
                     if (ring.lap) ok = mbar_wait_relaxed(w_empty + 8 * ring.slot, ring.empty_parity(), abort_flag, p.status, 51);
                     if (!ok) break;
+                    if (i - u.kb0 == p.test_skip_kblock) continue;    // test hook: this block never arrives, its consumers' waits run out
                     mbar_arrive_expect_tx(w_full + 8 * ring.slot, C::W_STAGE_BYTES);
                     tma_load_3d(smem_u32(sW) + ring.slot * C::W_STAGE_BYTES, &tmap_w, i * kW4BlockBytes, row, u.expert, w_full + 8 * ring.slot);
                 }
@@ -844,6 +846,7 @@ int launch_w4_umma(cudaStream_t stream, const W4Gemm& problem, int dtype, void* 
     GemmParams hooks{};
     apply_test_hooks(hooks);
     q.wait_budget = hooks.wait_budget;
+    q.test_skip_kblock = hooks.test_skip_kblock;
     return dtype == BGEMM_DT_F16 ? umma_dtype<__half>(stream, tw, tx, q) : umma_dtype<__nv_bfloat16>(stream, tw, tx, q);
 }
 

@@ -396,9 +396,9 @@ int bgemm_moe_combine(void* stream, const void* y, int dtype, int64_t slots_tota
 
 /* Every wait inside the kernels is time-bounded (about 0.2 s of SM clock). A wait that runs out makes its kernel
  * drain and exit normally and records a small positive code in a per-device status word (11-18: tile-per-CTA
- * GEMM, 21-29: persistent GEMM; the number names the barrier that was not reached); the results of that launch
- * are then undefined. This call synchronises with the device, returns the word (0 = no wait
- * ever ran out) and clears it when `reset` is non-zero. The reference has no counterpart: its kernels
+ * GEMM, 21-29: persistent GEMM, 31: streaming GEMM, 41-49: GEMM on SM pairs, 51-59: 4-bit products on the tensor
+ * cores; the number names the barrier that was not reached); the results of that launch are then undefined. This call
+ * synchronises with the device, returns the word (0 = no wait ever ran out) and clears it when `reset` is non-zero. The reference has no counterpart: its kernels
  * have no inter-thread waits beyond __syncthreads (kernel_matmul.cuh:458-459,507-508).                   */
 int bgemm_device_status(int reset);
 
@@ -406,8 +406,8 @@ int bgemm_device_status(int reset);
  * are process-wide and apply to the GEMM launches that follow: `wait_budget_clocks` > 0 shortens every bounded wait
  * to that many SM clocks (0 = back to the default), and `skip_kblock` >= 0 makes the weight producer of every CTA
  * of the tensor-core kernels withhold the weight tile of that K block (counted from the start of the CTA's own K
- * range; -1 = none), so that the consumers' waits run out: the launch then drains, exits normally and reports a
- * code through bgemm_device_status; its results are undefined. Nothing faults or hangs.                     */
+ * range; for the 4-bit products a block is 128 columns, counted from the start of each tile; -1 = none), so that the
+ * consumers' waits run out: the launch then drains, exits normally and reports a code through bgemm_device_status; its results are undefined. Nothing faults or hangs.                     */
 void bgemm_debug_set_wait_test(int64_t wait_budget_clocks, int skip_kblock);
 
 /* Test and tuning hook (no counterpart in the reference): which launches the kernel on SM pairs (256 x 256 tiles,
