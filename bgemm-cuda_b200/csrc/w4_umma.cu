@@ -201,8 +201,8 @@ struct UHalves {
     }
 };
 
-// VEC: the result's pitch is a multiple of 16 bytes. Where it is not, octets go out in as few pieces as their address allows (14340 x 4096 on
-// 2000 rows 170 us, value by value 225 to 250); as a branch of one kernel that cost the others up to a tenth (4096 x 256 on 4096 rows 27.7 -> 30.4).
+// VEC: the result's rows start on 16-byte boundaries, by their first and their pitch. Where they do not, octets go out in as few pieces as their address allows (14340 x 4096 on
+// 2000 rows 170 us, 14336 x 4096 from an odd address 165 to 185; value by value 225 to 250); as a branch of one kernel that cost the others up to a tenth (4096 x 256 on 4096 rows 27.7 -> 30.4).
 template <typename T, int GW, bool GATHER, bool VEC>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kUThreads, 1)
 w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ UXMaps tmap_x, const W4UmmaParams p) {
@@ -576,7 +576,6 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
         const int et = (warp & 3) * 32 + lane;                // weight row == tensor-memory lane; also the thread's number in its group
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         uint8_t* stage = sOut + hw * C::STAGED * C::PITCH;
-        const bool vec = p.g.out_ld % 8 == 0 && (reinterpret_cast<uintptr_t>(p.g.out) & 15) == 0;
         UHalves h;
         for (int t = cid; t < total; t += ncl) {
             const UTile u = plan.get(t);
@@ -627,7 +626,7 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
                             if constexpr (!VEC) {
                                 const uint32_t w[4] = {v.x, v.y, v.z, v.w};
                                 store_octet(dst, p.g.M - m0 - m, w);
-                            } else if (vec && m0 + m + 8 <= p.g.M) {
+                            } else if (m0 + m + 8 <= p.g.M) {
                                 *reinterpret_cast<uint4*>(dst) = v;
                             } else {
                                 const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -802,7 +801,7 @@ static int umma_groups(cudaStream_t stream, const CUtensorMap& tw, const UXMaps&
 }
 template <typename T>
 static int umma_dtype(cudaStream_t stream, const CUtensorMap& tw, const UXMaps& tx, const W4UmmaParams& p) {
-    const bool vec = p.g.out_ld % 8 == 0;
+    const bool vec = p.g.out_ld % 8 == 0 && reinterpret_cast<uintptr_t>(p.g.out) % 16 == 0;
     if (p.g.rows) return vec ? umma_groups<T, true, true>(stream, tw, tx, p) : umma_groups<T, true, false>(stream, tw, tx, p);
     return vec ? umma_groups<T, false, true>(stream, tw, tx, p) : umma_groups<T, false, false>(stream, tw, tx, p);
 }
