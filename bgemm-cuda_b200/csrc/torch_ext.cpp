@@ -343,6 +343,7 @@ void check_group(int64_t group, const char* where) { TORCH_CHECK(group == 32 || 
 
 void no_grad_only(const torch::Tensor& t, const char* where) {
     TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), where, ": forward only (no gradient): call it under torch.no_grad() or detach its input");
+    TORCH_CHECK(!t._fw_grad(0).defined(), where, ": forward only (no tangent): detach its input");      // the result would carry none, which reads as zero
 }
 
 // plane [.., M, row bytes], scales [.., M, groups], zeros the same as scales; all contiguous, on x's device

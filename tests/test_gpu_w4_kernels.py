@@ -404,3 +404,27 @@ def test_one_expert_takes_the_kernel_of_the_dense_product(L, M, K, n):
     assert torch.equal(L.w4a16_grouped_forward(x, plane, scales, zeros, ragged([n]), None, 64), dense)
     assert [b - a for a, b in zip(before, middle)] == [b - a for a, b in zip(middle, calls())]
     assert bool((dense == (exact if middle[0] > before[0] else off)).all())
+
+
+def test_a_tangent_is_refused(L):
+    """Forward-mode: the results carry no tangent, which autograd would take for zero."""
+    import bgemm_linear as N
+    from torch.autograd import forward_ad as F
+
+    g = gen(31)
+    plane, scales, zeros = matrix((2,), 64, 64, 64, torch.float16, True, g)
+    x = torch.randn(4, 64, generator=g, device="cuda").half()
+    off, logits = ragged([2, 2]), torch.randn(4, 2, generator=g, device="cuda")
+    weights, _, _, _, slots = L.moe_route(logits, 1)
+    out = torch.zeros(4, 64, dtype=torch.float16, device="cuda")
+    linear, experts = N.W4Linear(x.repeat(16, 1)), N.W4Experts(torch.randn(2, 64, 64, device="cuda").half(), torch.randn(2, 64, 32, device="cuda").half(), 1)
+    with F.dual_level(), torch.no_grad():
+        dual = lambda t: F.make_dual(t, torch.ones_like(t))      # noqa: E731
+        for call in (lambda: L.w4_quantize(dual(x), 64), lambda: L.w4_dequantize(plane, dual(scales), zeros, 64, 64),
+                     lambda: L.w4a16_linear_forward(dual(x), plane[0], scales[0], zeros[0], 64), lambda: L.w4a16_linear_forward(x, plane[0], dual(scales[0]), zeros[0], 64),
+                     lambda: L.w4a16_grouped_forward(dual(x), plane, scales, zeros, off, None, 64), lambda: L.w4a16_grouped_forward(x, plane, scales, zeros, off, None, 64, dual(out)),
+                     lambda: L.moe_route(dual(logits), 1), lambda: L.moe_combine(dual(x), slots, weights), lambda: L.moe_combine(x, slots, dual(weights)),
+                     lambda: linear(dual(x)), lambda: experts(dual(x), logits), lambda: experts(x, dual(logits))):
+            with pytest.raises(RuntimeError):
+                call()
+        assert linear(x).shape == experts(x, logits).shape == (4, 64)      # inputs without one are served
