@@ -129,9 +129,16 @@ def launch_count() -> int:
 
 
 def _require_cuda(*ts):
+    """CUDA tensors of one device: a kernel runs on one, and a pointer into another GPU's memory faults there."""
+    device = None
     for t in ts:
-        if t is not None and not t.is_cuda:
+        if t is None:
+            continue
+        if not t.is_cuda:
             raise ValueError("expected a CUDA tensor (this library has no CPU path)")
+        device = device or t.device
+        if t.device != device:
+            raise ValueError(f"all tensors must be on one device, got {device} and {t.device}")
 
 
 def pack_weights(w: torch.Tensor, wbit_mode: int = WBIT_NEGATIVE, want_rowpop: bool = False, want_alpha: bool = False):
@@ -385,8 +392,9 @@ def w4_dequantize(plane: torch.Tensor, scales: torch.Tensor, zeros: "torch.Tenso
 def w4a16_gemm(x: torch.Tensor, plane: torch.Tensor, scales: torch.Tensor, zeros: "torch.Tensor | None" = None, group: int = 128,
                out: "torch.Tensor | None" = None) -> torch.Tensor:
     """x [N, K] (the scales' type) times a 4-bit matrix -> [N, M]; `out`: a row-major [N, M] tensor, any row pitch."""
+    _require_cuda(x, plane)
     _w4_check(plane, scales, zeros, x.shape[1], group)
-    if not x.is_cuda or x.dtype != scales.dtype or plane.dim() != 2:
+    if x.dtype != scales.dtype or plane.dim() != 2:
         raise ValueError("x must be a CUDA tensor [N, K] of the scales' type and the plane [M, bytes]")
     x, ld = _rows(x)
     N, M = x.shape[0], plane.shape[0]
@@ -405,8 +413,8 @@ def w4a16_gemm(x: torch.Tensor, plane: torch.Tensor, scales: torch.Tensor, zeros
 def w4a16_grouped_gemm(x: torch.Tensor, plane: torch.Tensor, scales: torch.Tensor, zeros: "torch.Tensor | None", offsets: torch.Tensor,
                        rows: "torch.Tensor | None" = None, group: int = 128, out: "torch.Tensor | None" = None) -> torch.Tensor:
     """The same product by expert (plane [E, M, bytes], offsets int32 [E + 1]); rows of the result behind offsets[E] are not written."""
+    _require_cuda(x, plane, offsets, rows)
     _w4_check(plane, scales, zeros, x.shape[1], group)
-    _require_cuda(x, offsets, rows)
     E, M = plane.shape[0], plane.shape[1]
     if x.dtype != scales.dtype or plane.dim() != 3 or offsets.dtype != torch.int32 or offsets.numel() != E + 1 or not offsets.is_contiguous():
         raise ValueError("x must have the scales' type, the plane [E, M, bytes] and offsets int32 [E + 1]")
