@@ -11,6 +11,7 @@ import os
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 _DIR = Path(__file__).resolve().parent
 _LIB_PATH = Path(os.environ.get("BGEMM_B200_LIB", _DIR / "libbgemm_b200.so"))
@@ -343,6 +344,13 @@ def linear_forward(weight_f16: torch.Tensor, acts_f16: torch.Tensor, op: int = O
 
 
 # ---- 4-bit weights and expert routing ----
+def _forward_only(*ts):
+    """The results carry no gradient, neither backward nor forward-mode: refused where one is asked for."""
+    for t in ts:
+        if t is not None and ((t.requires_grad and torch.is_grad_enabled()) or forward_ad.unpack_dual(t).tangent is not None):
+            raise ValueError("forward only (no gradient): call it under torch.no_grad() with an input that carries no tangent, or detach the input")
+
+
 def _w4_check(plane, scales, zeros, K, group):
     _require_cuda(plane, scales, zeros)
     if not (plane.is_contiguous() and scales.is_contiguous() and plane.dtype == torch.uint8 and scales.dtype in (torch.float16, torch.bfloat16)):
@@ -351,6 +359,7 @@ def _w4_check(plane, scales, zeros, K, group):
         raise ValueError("plane must be [.., M, w4_row_bytes(K)] and scales [.., M, ceil(K / group)]")
     if zeros is not None and not (zeros.is_contiguous() and zeros.dtype == torch.uint8 and zeros.shape == scales.shape):
         raise ValueError("zeros must be contiguous uint8 of the scales' shape")
+    _forward_only(scales)
 
 
 def _rows(x):
@@ -365,6 +374,7 @@ def w4_quantize(w: torch.Tensor, group: int = 128, symmetric: bool = False, scal
     _require_cuda(w)
     if w.dim() not in (2, 3) or w.numel() == 0:
         raise ValueError("expected a non-empty [M, K] or [B, M, K] tensor")
+    _forward_only(w)
     if w.stride(-1) != 1 or (w.shape[-2] > 1 and w.stride(-2) < w.shape[-1]):
         w = w.contiguous()
     M, K = w.shape[-2:]
@@ -396,6 +406,7 @@ def w4a16_gemm(x: torch.Tensor, plane: torch.Tensor, scales: torch.Tensor, zeros
     _w4_check(plane, scales, zeros, x.shape[1], group)
     if x.dtype != scales.dtype or plane.dim() != 2:
         raise ValueError("x must be a CUDA tensor [N, K] of the scales' type and the plane [M, bytes]")
+    _forward_only(x, out)
     x, ld = _rows(x)
     N, M = x.shape[0], plane.shape[0]
     if out is None:
@@ -420,6 +431,7 @@ def w4a16_grouped_gemm(x: torch.Tensor, plane: torch.Tensor, scales: torch.Tenso
         raise ValueError("x must have the scales' type, the plane [E, M, bytes] and offsets int32 [E + 1]")
     if rows is not None and (rows.dtype != torch.int32 or rows.dim() != 1 or not rows.is_contiguous()):
         raise ValueError("rows must be a contiguous int32 tensor")
+    _forward_only(x, out)
     x, ld = _rows(x)
     slots = x.shape[0] if rows is None else rows.numel()
     if out is None:
@@ -438,6 +450,7 @@ def w4a16_grouped_gemm(x: torch.Tensor, plane: torch.Tensor, scales: torch.Tenso
 def moe_route(logits: torch.Tensor, top_k: int, renormalize: bool = True):
     """[T, E] -> (weights fp32 [T, k], experts int32 [T, k], offsets int32 [E + 1], rows int32 [T k], slots int32 [T, k])."""
     _require_cuda(logits)
+    _forward_only(logits)
     x, ld = _rows(logits)
     T, E = x.shape
     ints = dict(dtype=torch.int32, device=x.device)
@@ -457,6 +470,7 @@ def moe_combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor) -> 
     _require_cuda(y, slots, weights)
     if slots.dtype != torch.int32 or weights.dtype != torch.float32 or slots.shape != weights.shape or not (slots.is_contiguous() and weights.is_contiguous()):
         raise ValueError("slots (int32) and weights (float32) must be contiguous tensors of one shape [T, k]")
+    _forward_only(y, weights)
     y, ld = _rows(y)
     T, M = slots.shape[0], y.shape[1]
     out = torch.empty((T, M), dtype=y.dtype, device=y.device)

@@ -428,3 +428,31 @@ def test_a_tangent_is_refused(L):
             with pytest.raises(RuntimeError):
                 call()
         assert linear(x).shape == experts(x, logits).shape == (4, 64)      # inputs without one are served
+
+
+def test_the_ctypes_binding_refuses_gradients_too(L):
+    import bgemm_b200 as B
+    from torch.autograd import forward_ad as F
+
+    g = gen(32)
+    plane, scales, zeros = matrix((2,), 64, 64, 64, torch.float16, True, g)
+    x = torch.randn(4, 64, generator=g, device="cuda").half()
+    off, logits = ragged([2, 2]), torch.randn(4, 2, generator=g, device="cuda")
+    weights, _, _, _, slots = B.moe_route(logits, 1)
+    out = torch.zeros(4, 64, dtype=torch.float16, device="cuda")
+    calls = lambda v: [lambda: B.w4_quantize(v(x), 64), lambda: B.w4_dequantize(plane, v(scales), zeros, 64, 64),      # noqa: E731
+                       lambda: B.w4a16_gemm(v(x), plane[0], scales[0], zeros[0], 64), lambda: B.w4a16_gemm(x, plane[0], v(scales[0]), zeros[0], 64),
+                       lambda: B.w4a16_gemm(x, plane[0], scales[0], zeros[0], 64, v(out)), lambda: B.w4a16_grouped_gemm(v(x), plane, scales, zeros, off, None, 64),
+                       lambda: B.w4a16_grouped_gemm(x, plane, scales, zeros, off, None, 64, v(out)), lambda: B.moe_route(v(logits), 1), lambda: B.moe_combine(v(x), slots, weights),
+                       lambda: B.moe_combine(x, slots, v(weights))]
+    learnt = lambda t: t.clone().requires_grad_(True)            # noqa: E731
+    for call in calls(learnt):
+        with pytest.raises(ValueError):
+            call()
+    with torch.no_grad():
+        for call in calls(learnt):
+            call()
+        with F.dual_level():
+            for call in calls(lambda t: F.make_dual(t, torch.ones_like(t))):
+                with pytest.raises(ValueError):
+                    call()
