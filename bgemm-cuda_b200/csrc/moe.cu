@@ -115,7 +115,7 @@ __device__ __forceinline__ void route_tokens(const void* logits, long long ld, l
                 if (!renormalize && top[p] != 0u) {
                     if (best[p] < INFINITY) {
 #pragma unroll
-                        for (int i = 0; i < V; i++) total[p] += __expf(value[p][i] - best[p]);
+                        for (int i = 0; i < V; i++) total[p] += expf(value[p][i] - best[p]);      // the function of the numerators
                     } else {                     // +inf: equal logits differ by 0
 #pragma unroll
                         for (int i = 0; i < V; i++) total[p] += value[p][i] == best[p] ? 1.f : 0.f;
