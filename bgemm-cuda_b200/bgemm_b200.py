@@ -56,6 +56,7 @@ lib.bgemm_w1a16_gemm.argtypes = [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _in
 lib.bgemm_gemm_to_acts.argtypes = [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _int, _vp, _int, _vp, _vp, _int, _vp, _sz, _i64]
 lib.bgemm_gemm_to_acts_ex.argtypes = [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _int, _vp, _int, _vp, _vp, _int, _vp, _sz, _i64, _int]
 FLAG_SUMS_ZEROED = 4
+FLAG_EXACT_WEIGHTS = 8
 lib.bgemm_gemm_workspace_bytes.restype = _sz
 lib.bgemm_gemm_workspace_bytes.argtypes = [_i64, _i64, _i64, _int, _i64]
 lib.bgemm_debug_set_pair_kernel.restype = None
@@ -75,9 +76,11 @@ lib.bgemm_w4_row_bytes.argtypes = [_i64]
 lib.bgemm_w4_quantize.argtypes = [_vp, _vp, _int, _i64, _i64, _i64, _int, _int, _int, _vp, _vp, _vp, _i64, _i64]
 lib.bgemm_w4_dequantize.argtypes = [_vp, _vp, _i64, _i64, _int, _vp, _vp, _int, _vp]
 lib.bgemm_w4a16_gemm.argtypes = [_vp, _vp, _i64, _i64, _int, _vp, _vp, _vp, _i64, _int, _i64, _vp, _i64, _vp, _sz]
+lib.bgemm_w4a16_gemm_ex.argtypes = lib.bgemm_w4a16_gemm.argtypes + [_int]
 lib.bgemm_w4a16_workspace_bytes.restype = _sz
 lib.bgemm_w4a16_workspace_bytes.argtypes = [_i64, _i64, _i64, _i64]
 lib.bgemm_w4a16_grouped_gemm.argtypes = [_vp, _vp, _i64, _i64, _i64, _int, _vp, _vp, _vp, _i64, _i64, _int, _vp, _vp, _i64, _vp, _i64, _vp, _sz]
+lib.bgemm_w4a16_grouped_gemm_ex.argtypes = lib.bgemm_w4a16_grouped_gemm.argtypes + [_int]
 lib.bgemm_moe_route_workspace_bytes.restype = _sz
 lib.bgemm_moe_route_workspace_bytes.argtypes = [_i64, _i64]
 lib.bgemm_moe_route.argtypes = [_vp, _vp, _int, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp, _vp, _vp, _vp, _sz]
@@ -400,8 +403,8 @@ def w4_dequantize(plane: torch.Tensor, scales: torch.Tensor, zeros: "torch.Tenso
 
 
 def w4a16_gemm(x: torch.Tensor, plane: torch.Tensor, scales: torch.Tensor, zeros: "torch.Tensor | None" = None, group: int = 128,
-               out: "torch.Tensor | None" = None) -> torch.Tensor:
-    """x [N, K] (the scales' type) times a 4-bit matrix -> [N, M]; `out`: a row-major [N, M] tensor, any row pitch."""
+               out: "torch.Tensor | None" = None, exact: bool = False) -> torch.Tensor:
+    """x [N, K] (the scales' type) times a 4-bit matrix -> [N, M]; `out`: a row-major [N, M] tensor, any row pitch. exact: no weight is rounded at any N."""
     _require_cuda(x, plane)
     _w4_check(plane, scales, zeros, x.shape[1], group)
     if x.dtype != scales.dtype or plane.dim() != 2:
@@ -413,16 +416,16 @@ def w4a16_gemm(x: torch.Tensor, plane: torch.Tensor, scales: torch.Tensor, zeros
         out = torch.empty((N, M), dtype=x.dtype, device=x.device)
     elif out.shape != (N, M) or out.dtype != x.dtype or out.stride(1) != 1 or out.device != x.device:
         raise ValueError("out must be a row-major [N, M] tensor of x's type")
-    need = lib.bgemm_w4a16_workspace_bytes(1, M, x.shape[1], N)
+    need = 0 if exact else lib.bgemm_w4a16_workspace_bytes(1, M, x.shape[1], N)
     ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     with torch.cuda.device(x.device):
-        check(lib.bgemm_w4a16_gemm(_stream(), plane.data_ptr(), M, x.shape[1], group, scales.data_ptr(), _ptr(zeros), x.data_ptr(), ld, dtype_code(x), N,
-                                   out.data_ptr(), out.stride(0) if N > 1 else M, _ptr(ws), need), "bgemm_w4a16_gemm")
+        check(lib.bgemm_w4a16_gemm_ex(_stream(), plane.data_ptr(), M, x.shape[1], group, scales.data_ptr(), _ptr(zeros), x.data_ptr(), ld, dtype_code(x), N,
+                                   out.data_ptr(), out.stride(0) if N > 1 else M, _ptr(ws), need, FLAG_EXACT_WEIGHTS if exact else 0), "bgemm_w4a16_gemm")
     return out
 
 
 def w4a16_grouped_gemm(x: torch.Tensor, plane: torch.Tensor, scales: torch.Tensor, zeros: "torch.Tensor | None", offsets: torch.Tensor,
-                       rows: "torch.Tensor | None" = None, group: int = 128, out: "torch.Tensor | None" = None) -> torch.Tensor:
+                       rows: "torch.Tensor | None" = None, group: int = 128, out: "torch.Tensor | None" = None, exact: bool = False) -> torch.Tensor:
     """The same product by expert (plane [E, M, bytes], offsets int32 [E + 1]); rows of the result behind offsets[E] are not written."""
     _require_cuda(x, plane, offsets, rows)
     _w4_check(plane, scales, zeros, x.shape[1], group)
@@ -438,12 +441,12 @@ def w4a16_grouped_gemm(x: torch.Tensor, plane: torch.Tensor, scales: torch.Tenso
         out = torch.empty((slots, M), dtype=x.dtype, device=x.device)
     elif out.shape != (slots, M) or out.dtype != x.dtype or out.stride(1) != 1 or out.device != x.device:
         raise ValueError("out must be a row-major [slots, M] tensor of x's type")
-    need = lib.bgemm_w4a16_workspace_bytes(E, M, x.shape[1], slots)
+    need = 0 if exact else lib.bgemm_w4a16_workspace_bytes(E, M, x.shape[1], slots)
     ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     with torch.cuda.device(x.device):
-        check(lib.bgemm_w4a16_grouped_gemm(_stream(), plane.data_ptr(), E, M, x.shape[1], group, scales.data_ptr(), _ptr(zeros), x.data_ptr(), x.shape[0], ld,
+        check(lib.bgemm_w4a16_grouped_gemm_ex(_stream(), plane.data_ptr(), E, M, x.shape[1], group, scales.data_ptr(), _ptr(zeros), x.data_ptr(), x.shape[0], ld,
                                            dtype_code(x), offsets.data_ptr(), _ptr(rows), slots, out.data_ptr(), out.stride(0) if slots > 1 else M, _ptr(ws),
-                                           need), "bgemm_w4a16_grouped_gemm")
+                                           need, FLAG_EXACT_WEIGHTS if exact else 0), "bgemm_w4a16_grouped_gemm")
     return out
 
 

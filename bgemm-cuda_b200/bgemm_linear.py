@@ -516,20 +516,22 @@ class W4Linear(nn.Module):
     a zero point) per row and group of ``group_size`` (32, 64 or 128) columns.
 
     ``weight`` [out, in] is quantised once, on the GPU (fp16 or bf16: the layer then takes and returns that type; fp32 weights
-    make an fp16 layer, or a bf16 one with ``dtype=torch.bfloat16``). Any sizes; any number of rows: up to eight the product is a
-    weight-streaming kernel that never rounds a weight, from a few dozen on the tensor cores take it (csrc/w4_stream.cu,
-    csrc/w4_umma.cu). Forward only: calling it while a gradient is asked of x raises.
+    make an fp16 layer, or a bf16 one with ``dtype=torch.bfloat16``). Any sizes; any number of rows: up to eight, and more while
+    the passes over the matrix stay small, the product is a weight-streaming kernel that never rounds a weight; others go to the tensor cores, where
+    each weight is first rounded to that type (csrc/w4_stream.cu, csrc/w4_umma.cu; include/bgemm_b200.h has the limit). With ``exact`` no
+    weight is rounded at any number of rows, so that a row meets the same weights in any batch (about ten times the time on 2000 rows).
+    Forward only: calling it while a gradient is asked of x raises.
 
     Buffers: ``plane`` (codes, include/bgemm_b200.h has the layout), ``scales``, ``zeros`` (absent when symmetric), ``bias``.
     """
 
     def __init__(self, weight: torch.Tensor, group_size: int = 128, symmetric: bool = False, bias: "torch.Tensor | None" = None,
-                 dtype: "torch.dtype | None" = None):
+                 dtype: "torch.dtype | None" = None, exact: bool = False):
         super().__init__()
         if weight.dim() != 2:
             raise ValueError("W4Linear: weight must be [out_features, in_features]")
         self.out_features, self.in_features = weight.shape
-        self.group_size, self.symmetric = group_size, symmetric
+        self.group_size, self.symmetric, self.exact = group_size, symmetric, exact
         plane, scales, zeros = _w4_quantize(weight, group_size, symmetric, dtype)
         self.register_buffer("plane", plane)
         self.register_buffer("scales", scales)
@@ -544,7 +546,7 @@ class W4Linear(nn.Module):
         if x.dim() < 1 or x.shape[-1] != self.in_features:
             raise ValueError(f"W4Linear: x must be [.., {self.in_features}]")
         lead = x.shape[:-1]
-        out = lowbit_kernel.w4a16_linear_forward(x.reshape(-1, self.in_features), self.plane, self.scales, self.zeros, self.group_size)
+        out = lowbit_kernel.w4a16_linear_forward(x.reshape(-1, self.in_features), self.plane, self.scales, self.zeros, self.group_size, self.exact)
         out = out.reshape(*lead, self.out_features)
         return out if self.bias is None else out + self.bias
 
@@ -566,18 +568,19 @@ class W4Experts(nn.Module):
     ``gate_up`` [E, 2 I, H] (gate rows first) and ``down`` [E, H, I] are quantised once like W4Linear's weight. ``forward``
     takes the tokens [.., H] and the router's logits [.., E]: routing, both products and the weighted sum stay on the device, nothing is
     read back, so a captured forward can be replayed with other tokens. Experts whose logit is -inf are never chosen; a token whose
-    logits are all -inf (padding) gets zeros and costs nothing. Forward only.
+    logits are all -inf (padding) gets zeros and costs nothing. The gate's silu, its product with up and both products' results are rounded to
+    the weights' 16-bit type. ``exact`` as in W4Linear. Forward only.
     """
 
     def __init__(self, gate_up: torch.Tensor, down: torch.Tensor, top_k: int, renormalize: bool = True, group_size: int = 128,
-                 symmetric: bool = False, dtype: "torch.dtype | None" = None):
+                 symmetric: bool = False, dtype: "torch.dtype | None" = None, exact: bool = False):
         super().__init__()
         if gate_up.dim() != 3 or down.dim() != 3 or gate_up.shape[0] != down.shape[0] or gate_up.shape[1] != 2 * down.shape[2] or gate_up.shape[2] != down.shape[1]:
             raise ValueError("W4Experts: gate_up must be [E, 2 I, H] and down [E, H, I]")
         self.num_experts, self.hidden_size, self.intermediate_size = down.shape
         if not 1 <= top_k <= min(self.num_experts, 32):
             raise ValueError("W4Experts: 1 <= top_k <= min(E, 32) required")
-        self.top_k, self.renormalize, self.group_size = top_k, renormalize, group_size
+        self.top_k, self.renormalize, self.group_size, self.exact = top_k, renormalize, group_size, exact
         for name, w in (("gate_up", gate_up), ("down", down)):
             plane, scales, zeros = _w4_quantize(w, group_size, symmetric, dtype)
             self.register_buffer(name + "_plane", plane)
@@ -592,9 +595,9 @@ class W4Experts(nn.Module):
         if logits.dim() < 1 or logits.shape[:-1] != lead or logits.shape[-1] != self.num_experts:
             raise ValueError("W4Experts: logits must have x's leading sizes and one value per expert")
         weights, _, offsets, rows, slots = lowbit_kernel.moe_route(logits.reshape(-1, self.num_experts), self.top_k, self.renormalize)
-        h = lowbit_kernel.w4a16_grouped_forward(x2, self.gate_up_plane, self.gate_up_scales, self.gate_up_zeros, offsets, rows, self.group_size)
+        h = lowbit_kernel.w4a16_grouped_forward(x2, self.gate_up_plane, self.gate_up_scales, self.gate_up_zeros, offsets, rows, self.group_size, exact=self.exact)
         # rows behind offsets[E] are not written by the products, not read by the next one and named by no slot
         gate, up = h.split(self.intermediate_size, dim=-1)
         h = nn.functional.silu(gate) * up
-        y = lowbit_kernel.w4a16_grouped_forward(h, self.down_plane, self.down_scales, self.down_zeros, offsets, None, self.group_size)
+        y = lowbit_kernel.w4a16_grouped_forward(h, self.down_plane, self.down_scales, self.down_zeros, offsets, None, self.group_size, exact=self.exact)
         return lowbit_kernel.moe_combine(y, slots, weights).reshape(*lead, self.hidden_size)

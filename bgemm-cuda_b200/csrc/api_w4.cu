@@ -86,8 +86,8 @@ bool on_tensor_cores(const W4Gemm& p) {
     return rows > 8 && experts * (rows / 8 + 0.4) * matrix > 45e6;
 }
 
-int run(cudaStream_t stream, const W4Gemm& p, int dtype, void* workspace, size_t workspace_bytes) {
-    const bool tensor = on_tensor_cores(p);
+int run(cudaStream_t stream, const W4Gemm& p, int dtype, void* workspace, size_t workspace_bytes, int flags) {
+    const bool tensor = !(flags & BGEMM_FLAG_EXACT_WEIGHTS) && on_tensor_cores(p);
     g_w4_calls[tensor].fetch_add(1, std::memory_order_relaxed);
     if (!tensor) return launch_w4_stream(stream, p, dtype);
     const size_t need = w4_umma_workspace(p);
@@ -134,16 +134,30 @@ size_t bgemm_w4a16_workspace_bytes(int64_t E, int64_t M, int64_t K, int64_t slot
 
 int bgemm_w4a16_gemm(void* stream, const void* plane, int64_t M, int64_t K, int group, const void* scales, const uint8_t* zeros, const void* x,
                      int64_t x_ld, int dtype, int64_t N, void* out, int64_t out_ld, void* workspace, size_t workspace_bytes) {
+    return bgemm_w4a16_gemm_ex(stream, plane, M, K, group, scales, zeros, x, x_ld, dtype, N, out, out_ld, workspace, workspace_bytes, 0);
+}
+
+int bgemm_w4a16_gemm_ex(void* stream, const void* plane, int64_t M, int64_t K, int group, const void* scales, const uint8_t* zeros, const void* x,
+                        int64_t x_ld, int dtype, int64_t N, void* out, int64_t out_ld, void* workspace, size_t workspace_bytes, int flags) {
+    if (flags & ~BGEMM_FLAG_EXACT_WEIGHTS) return BGEMM_ERR_ENUM;
     const int rc = check_gemm(plane, M, K, group, scales, x, x_ld, N, dtype, N, out, out_ld);
     if (rc) return rc;
     const W4Gemm p = problem(plane, 1, M, K, group, scales, zeros, x, x_ld, N, N, out, out_ld);
     if (!aligned(workspace, 256)) return BGEMM_ERR_ALIGN;
-    return run((cudaStream_t)stream, p, dtype, workspace, workspace_bytes);
+    return run((cudaStream_t)stream, p, dtype, workspace, workspace_bytes, flags);
 }
 
 int bgemm_w4a16_grouped_gemm(void* stream, const void* plane, int64_t E, int64_t M, int64_t K, int group, const void* scales, const uint8_t* zeros,
                              const void* x, int64_t x_rows, int64_t x_ld, int dtype, const int32_t* offsets, const int32_t* rows, int64_t slots,
                              void* out, int64_t out_ld, void* workspace, size_t workspace_bytes) {
+    return bgemm_w4a16_grouped_gemm_ex(stream, plane, E, M, K, group, scales, zeros, x, x_rows, x_ld, dtype, offsets, rows, slots, out, out_ld, workspace,
+                                       workspace_bytes, 0);
+}
+
+int bgemm_w4a16_grouped_gemm_ex(void* stream, const void* plane, int64_t E, int64_t M, int64_t K, int group, const void* scales, const uint8_t* zeros,
+                                const void* x, int64_t x_rows, int64_t x_ld, int dtype, const int32_t* offsets, const int32_t* rows, int64_t slots,
+                                void* out, int64_t out_ld, void* workspace, size_t workspace_bytes, int flags) {
+    if (flags & ~BGEMM_FLAG_EXACT_WEIGHTS) return BGEMM_ERR_ENUM;
     if (!offsets) return BGEMM_ERR_NULL;
     const int rc = check_gemm(plane, M, K, group, scales, x, x_ld, x_rows, dtype, slots, out, out_ld);
     if (rc) return rc;
@@ -152,7 +166,7 @@ int bgemm_w4a16_grouped_gemm(void* stream, const void* plane, int64_t E, int64_t
     W4Gemm p = problem(plane, (int)E, M, K, group, scales, zeros, x, x_ld, x_rows, slots, out, out_ld);
     p.offsets = offsets;
     p.rows = rows;
-    return run((cudaStream_t)stream, p, dtype, workspace, workspace_bytes);
+    return run((cudaStream_t)stream, p, dtype, workspace, workspace_bytes, flags);
 }
 
 void bgemm_debug_set_w4_kernel(int mode) { g_w4_kernel.store(mode < -1 || mode > 1 ? -2 : mode, std::memory_order_relaxed); }

@@ -415,8 +415,8 @@ torch::Tensor rows_on_16_bytes(const torch::Tensor& x, int64_t products, double 
     return copy;
 }
 
-// x [N, K] times a 4-bit matrix -> [N, M] of x's type (which is the scales' type too).
-torch::Tensor w4a16_linear_forward(torch::Tensor x, torch::Tensor plane, torch::Tensor scales, c10::optional<torch::Tensor> zeros, int64_t group) {
+// x [N, K] times a 4-bit matrix -> [N, M] of x's type (which is the scales' type too). exact: no weight is rounded at any N (BGEMM_FLAG_EXACT_WEIGHTS).
+torch::Tensor w4a16_linear_forward(torch::Tensor x, torch::Tensor plane, torch::Tensor scales, c10::optional<torch::Tensor> zeros, int64_t group, bool exact) {
     const char* where = "w4a16_linear_forward";
     TORCH_CHECK(x.is_cuda() && x.dim() == 2 && plane.dim() == 2, where, ": x must be a CUDA tensor [N, K] and the plane [M, bytes]");
     TORCH_CHECK(x.scalar_type() == scales.scalar_type(), where, ": x and the scales must have one type");
@@ -428,11 +428,11 @@ torch::Tensor w4a16_linear_forward(torch::Tensor x, torch::Tensor plane, torch::
     auto out = fresh({N, M}, x.scalar_type());
     if (out.numel() == 0) return out;
     x = rows_on_16_bytes(x, N, (double)M * (double)K);
-    const size_t need = bgemm_w4a16_workspace_bytes(1, M, K, N);
+    const size_t need = exact ? 0 : bgemm_w4a16_workspace_bytes(1, M, K, N);
     torch::Tensor ws;
     if (need) ws = fresh({(int64_t)need}, at::kByte);
-    check(bgemm_w4a16_gemm(stream_of(x), plane.data_ptr(), M, K, (int)group, scales.data_ptr(), zeros_ptr(zeros), x.data_ptr(), N > 1 ? x.stride(0) : K,
-                           dtype_code(x), N, out.data_ptr(), M, need ? ws.data_ptr() : nullptr, need),
+    check(bgemm_w4a16_gemm_ex(stream_of(x), plane.data_ptr(), M, K, (int)group, scales.data_ptr(), zeros_ptr(zeros), x.data_ptr(), N > 1 ? x.stride(0) : K,
+                           dtype_code(x), N, out.data_ptr(), M, need ? ws.data_ptr() : nullptr, need, exact ? BGEMM_FLAG_EXACT_WEIGHTS : 0),
           "bgemm_w4a16_gemm");
     return out;
 }
@@ -440,7 +440,7 @@ torch::Tensor w4a16_linear_forward(torch::Tensor x, torch::Tensor plane, torch::
 // The same product by expert: plane [E, M, bytes], offsets int32 [E + 1], rows int32 [slots] or None (slot s reads row s of x).
 // Rows of the result behind offsets[E] are not written; `out` gives a buffer [slots, M] to write into.
 torch::Tensor w4a16_grouped_forward(torch::Tensor x, torch::Tensor plane, torch::Tensor scales, c10::optional<torch::Tensor> zeros, torch::Tensor offsets,
-                                    c10::optional<torch::Tensor> rows, int64_t group, c10::optional<torch::Tensor> out_opt) {
+                                    c10::optional<torch::Tensor> rows, int64_t group, c10::optional<torch::Tensor> out_opt, bool exact) {
     const char* where = "w4a16_grouped_forward";
     TORCH_CHECK(x.is_cuda() && x.dim() == 2 && plane.dim() == 3, where, ": x must be a CUDA tensor [rows, K] and the plane [E, M, bytes]");
     TORCH_CHECK(x.scalar_type() == scales.scalar_type(), where, ": x and the scales must have one type");
@@ -470,13 +470,13 @@ torch::Tensor w4a16_grouped_forward(torch::Tensor x, torch::Tensor plane, torch:
         return out;
     }
     x = rows_on_16_bytes(x, slots, (double)M * (double)K * (double)std::min(slots, E));
-    const size_t need = bgemm_w4a16_workspace_bytes(E, M, K, slots);
+    const size_t need = exact ? 0 : bgemm_w4a16_workspace_bytes(E, M, K, slots);
     torch::Tensor ws;
     if (need) ws = fresh({(int64_t)need}, at::kByte);
-    check(bgemm_w4a16_grouped_gemm(stream_of(x), plane.data_ptr(), E, M, K, (int)group, scales.data_ptr(), zeros_ptr(zeros), x.data_ptr(), x.size(0),
+    check(bgemm_w4a16_grouped_gemm_ex(stream_of(x), plane.data_ptr(), E, M, K, (int)group, scales.data_ptr(), zeros_ptr(zeros), x.data_ptr(), x.size(0),
                                    x.size(0) > 1 ? x.stride(0) : K, dtype_code(x), offsets.data_ptr<int>(),
                                    rows.has_value() ? rows->data_ptr<int>() : nullptr, slots, out.data_ptr(), slots > 1 ? out.stride(0) : M,
-                                   need ? ws.data_ptr() : nullptr, need),
+                                   need ? ws.data_ptr() : nullptr, need, exact ? BGEMM_FLAG_EXACT_WEIGHTS : 0),
           "bgemm_w4a16_grouped_gemm");
     return out;
 }
@@ -571,10 +571,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("w4_dequantize", &w4_dequantize, "Values of a 4-bit plane in the scales' type.", py::arg("plane"), py::arg("scales"), py::arg("zeros"),
           py::arg("K"), py::arg("group_size") = 128);
     m.def("w4a16_linear_forward", &w4a16_linear_forward, "16-bit activations x 4-bit weights, fp32 accumulation.", py::arg("x"), py::arg("plane"),
-          py::arg("scales"), py::arg("zeros") = py::none(), py::arg("group_size") = 128);
+          py::arg("scales"), py::arg("zeros") = py::none(), py::arg("group_size") = 128, py::arg("exact") = false);
     m.def("w4a16_grouped_forward", &w4a16_grouped_forward, "The same product with one 4-bit matrix per expert.", py::arg("x"), py::arg("plane"),
           py::arg("scales"), py::arg("zeros"), py::arg("offsets"), py::arg("rows") = py::none(), py::arg("group_size") = 128,
-          py::arg("out") = py::none());
+          py::arg("out") = py::none(), py::arg("exact") = false);
     m.def("moe_route", &moe_route, "Top-k experts, their weights and the order by expert.", py::arg("logits"), py::arg("top_k"),
           py::arg("renormalize") = true);
     m.def("moe_combine", &moe_combine, "Weighted sum of the experts' rows of each token.", py::arg("y"), py::arg("slots"), py::arg("weights"));

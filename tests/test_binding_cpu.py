@@ -35,3 +35,14 @@ def test_every_product_and_routing_call_checks_its_tensors_together(B):
                  lambda: B.w4_dequantize(here, there, None, 64), lambda: B.moe_combine(here, there, here), lambda: B.moe_combine(here, here, there)):
         with pytest.raises(ValueError, match="one device"):
             call()
+
+
+def test_unknown_flags_are_refused_before_any_launch(B):
+    fake = 0x1000
+    before = B.launch_count()
+    for flags in (1, 2, 4, 16, 8 | 1, -1):
+        assert B.lib.bgemm_w4a16_gemm_ex(None, fake, 8, 64, 32, fake, None, fake, 64, 0, 2, fake, 8, None, 0, flags) == -4
+        assert B.lib.bgemm_w4a16_grouped_gemm_ex(None, fake, 4, 8, 64, 32, fake, None, fake, 2, 64, 0, fake, None, 2, fake, 8, None, 0, flags) == -4
+    assert B.lib.bgemm_w4a16_gemm_ex(None, None, 8, 64, 32, fake, None, fake, 64, 0, 2, fake, 8, None, 0, 8) == -1
+    assert B.lib.bgemm_w4a16_grouped_gemm_ex(None, fake, 0, 8, 64, 32, fake, None, fake, 2, 64, 0, fake, None, 2, fake, 8, None, 0, 8) == -2
+    assert B.launch_count() == before

@@ -456,3 +456,41 @@ def test_the_ctypes_binding_refuses_gradients_too(L):
             for call in calls(lambda t: F.make_dual(t, torch.ones_like(t))):
                 with pytest.raises(ValueError):
                     call()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("M,K,n", [(28672, 8192, 17), (4096, 4096, 200), (1000, 1024, 2000)])
+def test_exact_weights_at_any_number_of_rows(L, M, K, n, dtype):
+    """Without the flag these sizes meet rounded weights; with it none is rounded, in both bindings, dense and by expert."""
+    import bgemm_b200 as B
+
+    plane, scales, zeros, x, exact, off = telling(1, M, K, 128, n, DT[dtype])
+    index = torch.arange(n, device="cuda").int()
+    assert bool((L.w4a16_linear_forward(x, plane[0], scales[0], zeros[0], 128) == off).all())
+    before = calls()
+    for got in (L.w4a16_linear_forward(x, plane[0], scales[0], zeros[0], 128, exact=True), B.w4a16_gemm(x, plane[0], scales[0], zeros[0], 128, exact=True),
+                L.w4a16_grouped_forward(x, plane, scales, zeros, ragged([n]), None, 128, exact=True), B.w4a16_grouped_gemm(x, plane, scales, zeros, ragged([n]), index, 128, exact=True)):
+        assert bool((got == exact).all())
+    assert [b - a for a, b in zip(before, calls())] == [4, 0]
+
+
+def test_exact_layers(L):
+    """W4Linear and W4Experts with exact: real values within the bound that rounds no weight; the default takes the other kernel."""
+    import bgemm_linear as N
+
+    g = gen(41)
+    w = torch.randn(2048, 2048, generator=g, device="cuda").half() * 0.05
+    x = torch.randn(600, 2048, generator=g, device="cuda").half()
+    before = calls()
+    layer = N.W4Linear(w, exact=True)
+    check(layer(x), x, layer.plane, layer.scales, layer.zeros, 2048, 128, False)
+    assert [b - a for a, b in zip(before, calls())] == [1, 0]
+    N.W4Linear(w)(x)
+    assert [b - a for a, b in zip(before, calls())] == [1, 1]
+    gate_up, down = torch.randn(4, 1024, 1024, generator=g, device="cuda").half() * 0.05, torch.randn(4, 1024, 512, generator=g, device="cuda").half() * 0.05
+    logits = torch.randn(600, 4, generator=g, device="cuda")
+    before = calls()
+    N.W4Experts(gate_up, down, 2, exact=True)(x[:, :1024], logits)
+    assert [b - a for a, b in zip(before, calls())] == [2, 0]
+    N.W4Experts(gate_up, down, 2)(x[:, :1024], logits)
+    assert [b - a for a, b in zip(before, calls())] == [2, 2]
