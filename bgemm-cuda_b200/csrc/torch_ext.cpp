@@ -407,7 +407,10 @@ torch::Tensor w4_dequantize(torch::Tensor plane, torch::Tensor scales, c10::opti
 // The tensor-core path loads x by TMA, whose rows start on 16-byte boundaries, and the other kernel is slowed down by rows that do not
 // (28672 x 8190 on 8 rows 51 us, 36 with the copy): a copy with such a pitch where x has another one, and there are more rows than two
 // passes take or so many codes that the call lasts longer than the copy's ~6 us on the host (4096 x 4095 on 8 rows: 10 us as it is).
+// A product that names a few of many rows by index takes them where they lie: the copy is of the whole of x, 8.5 ns a row of 4095 columns, and a slot off
+// 16 bytes costs 0.3 us more on 4096 weight rows (40 slots of 20000 rows 38 us, 199 with the copy; 256 of 1100 31 with it, 127 without).
 torch::Tensor rows_on_16_bytes(const torch::Tensor& x, int64_t products, double codes) {
+    if (x.size(0) > 32 * products) return x;
     if ((products <= 16 && (products == 1 || codes < 64e6)) || (reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && (x.size(0) == 1 || x.stride(0) % 8 == 0))) return x;
     const int64_t K = x.size(1);
     auto copy = torch::empty({x.size(0), (K + 7) / 8 * 8}, x.options()).narrow(1, 0, K);

@@ -220,10 +220,12 @@ def test_grouped_rows_by_index(L, kernel, per, M, K):
         at += c
 
 
+@pytest.mark.parametrize("K", [256, 6000])
 @pytest.mark.parametrize("slots", [7, 30, 400])
-def test_grouped_leaves_other_rows_alone(L, kernel, slots):
+def test_grouped_leaves_other_rows_alone(L, kernel, slots, K):
+    """With the longer rows the tensor cores divide K, and the kernel that adds the parts up keeps to the experts' rows too."""
     g = gen(slots)
-    E, M, K, group = 3, 70, 256, 128
+    E, M, group = 3, 70, 128
     plane, scales, zeros = matrix((E,), M, K, group, torch.float16, True, g, 0, True)
     n = slots - 3
     offsets = torch.tensor([0, n // 3, n // 3, n], dtype=torch.int32, device="cuda")
@@ -494,3 +496,24 @@ def test_exact_layers(L):
     assert [b - a for a, b in zip(before, calls())] == [2, 0]
     N.W4Experts(gate_up, down, 2)(x[:, :1024], logits)
     assert [b - a for a, b in zip(before, calls())] == [2, 2]
+
+
+@pytest.mark.parametrize("n", [1, 9, 40])
+def test_a_few_rows_of_a_large_x_are_not_paid_for_by_all_of_it(L, n):
+    """Rows off 16-byte boundaries, named by index: read where they lie, no copy of x."""
+    g = gen(n)
+    M, K, T = 4096, 4095, 20000
+    plane, scales, zeros = matrix((4,), M, K, 128, torch.bfloat16, True, g)
+    x = torch.randn(T, K, generator=g, device="cuda").bfloat16()
+    index = torch.randint(0, T, (n,), generator=g, device="cuda", dtype=torch.int32)
+    off = ragged([n - n // 2, 0, n // 2, 0])
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    got = L.w4a16_grouped_forward(x, plane, scales, zeros, off, index, 128)
+    assert torch.cuda.max_memory_allocated() - held < x.numel() // 4
+    at = off.tolist()
+    for e in range(4):
+        if at[e + 1] > at[e]:
+            sl = slice(at[e], at[e + 1])
+            check(got[sl], x[index[sl].long()], plane[e], scales[e], zeros[e], K, 128, False)
