@@ -525,6 +525,8 @@ class W4Linear(nn.Module):
     Buffers: ``plane`` (codes, include/bgemm_b200.h has the layout), ``scales``, ``zeros`` (absent when symmetric), ``bias``.
     """
 
+    exact = False          # also for layers pickled before there was such a choice
+
     def __init__(self, weight: torch.Tensor, group_size: int = 128, symmetric: bool = False, bias: "torch.Tensor | None" = None,
                  dtype: "torch.dtype | None" = None, exact: bool = False):
         super().__init__()
@@ -571,6 +573,8 @@ class W4Experts(nn.Module):
     logits are all -inf (padding) gets zeros and costs nothing. The gate's silu, its product with up and both products' results are rounded to
     the weights' 16-bit type. ``exact`` as in W4Linear. Forward only.
     """
+
+    exact = False
 
     def __init__(self, gate_up: torch.Tensor, down: torch.Tensor, top_k: int, renormalize: bool = True, group_size: int = 128,
                  symmetric: bool = False, dtype: "torch.dtype | None" = None, exact: bool = False):

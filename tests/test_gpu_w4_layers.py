@@ -186,3 +186,49 @@ def test_layers_refuse_other_widths_and_types(N):
         with pytest.raises(ValueError):
             call()
     assert layer(x[:, :H], logits).shape == (4, H) and linear(x[0, :H]).shape == (2 * I,)
+
+
+def test_layers_saved_before_they_had_a_choice_of_arithmetic(N):
+    """A pickled layer has the attributes of its time: without `exact` it behaves as it did."""
+    import pickle
+
+    g = gen(16)
+    linear = N.W4Linear(torch.randn(64, 128, generator=g, device="cuda").half())
+    experts = N.W4Experts(torch.randn(4, 64, 64, generator=g, device="cuda").half(), torch.randn(4, 64, 32, generator=g, device="cuda").half(), 2)
+    x, logits = torch.randn(5, 128, generator=g, device="cuda").half(), torch.randn(5, 4, generator=g, device="cuda")
+    want = linear(x), experts(x[:, :64], logits)
+    for layer in (linear, experts):
+        del layer.exact
+    linear, experts = pickle.loads(pickle.dumps(linear)), pickle.loads(pickle.dumps(experts))
+    assert torch.equal(linear(x), want[0]) and torch.equal(experts(x[:, :64], logits), want[1])
+    with torch.inference_mode():
+        assert torch.equal(linear(x), want[0]) and torch.equal(experts(x[:, :64], logits), want[1])
+
+
+def test_the_first_call_of_a_process_may_be_a_captured_one():
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import sys; sys.path[:0] = [sys.argv[1]]
+import torch, lowbit_kernel as L
+g = torch.Generator(device="cuda").manual_seed(0)
+plane = torch.randint(0, 256, (4, 2048, 1024), generator=g, device="cuda", dtype=torch.uint8)
+scales = torch.ones(4, 2048, 16, device="cuda", dtype=torch.bfloat16)
+off, rows = torch.tensor([0, 100, 200, 300, 400], dtype=torch.int32, device="cuda"), torch.arange(400, device="cuda").int()
+x, logits = torch.randn(400, 2048, generator=g, device="cuda").bfloat16(), torch.randn(400, 64, generator=g, device="cuda")
+torch.cuda.synchronize()
+def calls():
+    r = L.moe_route(logits, 4)
+    return [L.w4a16_grouped_forward(x, plane, scales, None, off, rows, 128), L.w4a16_linear_forward(x[:3], plane[0], scales[0], None, 128), *r, L.moe_combine(x, r[4][:100], r[0][:100]),
+            *L.w4_quantize(x), L.w4_dequantize(plane, scales, None, 2048, 128)]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = calls()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, calls()))
+"""
+    root = Path(__file__).resolve().parent.parent / "bgemm-cuda_b200"
+    subprocess.run([sys.executable, "-c", code, str(root)], check=True, timeout=240)
