@@ -554,6 +554,14 @@ w4_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
 #pragma unroll
                         for (int e = 0; e < 16; e++) v[16 * q + e] = w4_pair<T>(word[e >> 2] >> (4 * (e & 3)), mz, s2, magic);
                     }
+                    // Codes behind K stand for zero: their activations are, but (q - z) s of what they hold may be no number of the type. (The test
+                    // costs 0 to 2 % of narrow tiles; once a block, on the codes, 28672 x 8192 on 16 rows in groups of 128 took 57.8 us against 54.4.)
+                    const int left = p.g.K - kb * kW4Block - half * 64;
+                    if (left < 64) {
+#pragma unroll
+                        for (int e = 0; e < 32; e++)
+                            if (2 * e + 1 >= left) v[e] = 2 * e < left ? v[e] & 0xffffu : 0u;
+                    }
                     if (half == 0) {
                         if (lap) ok = mbar_wait(empty + 8 * set, (lap - 1) & 1, abort_flag, p.status, 58);
                         ok = __all_sync(0xffffffffu, ok);

@@ -146,6 +146,23 @@ def test_zero_point_uses_its_low_four_bits(L, kernel, group):
     assert torch.equal(L.w4a16_linear_forward(x, plane, scales, zeros, group), L.w4a16_linear_forward(x, plane, scales, zeros | 0xF0, group))
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("K", [1, 31, 127, 130, 200, 257, 1000, 4095])
+def test_codes_behind_k_are_ignored(L, kernel, K, dtype, group):
+    """Whatever they hold, also where (q - z) s of such a code is beyond the type's numbers: fp16 scales of 6000, codes 0..2, padding 15."""
+    g = gen(K)
+    M, N = 130, 70
+    codes = torch.randint(0, 3, (M, K), generator=g, device="cuda")
+    scales = torch.full((M, -(-K // group)), 6000.0 if dtype == "fp16" else 2.0 ** 126, dtype=DT[dtype], device="cuda")
+    zeros = torch.zeros(scales.shape, dtype=torch.uint8, device="cuda")
+    x = rows(N, K, DT[dtype], g, True).zero_()
+    x[torch.arange(N, device="cuda"), torch.randint(0, K, (N,), generator=g, device="cuda")] = 0.5 if dtype == "fp16" else 2.0 ** -30
+    want = W.linear(x, W.values(W.pack(codes), scales, zeros, K, group)).to(DT[dtype])
+    assert bool(torch.isfinite(want).all())
+    assert torch.equal(L.w4a16_linear_forward(x, W.pack(codes, 15), scales, zeros, group), want)
+
+
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 @pytest.mark.parametrize("M,K,N,group", [(300, 2048, 40, 64), (256, 4096, 200, 32), (1001, 4100, 17, 128), (1300, 4096, 300, 128)])
 def test_divided_k(L, tensor, M, K, N, group, dtype):
