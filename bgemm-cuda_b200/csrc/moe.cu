@@ -8,7 +8,7 @@
 // Order: a counting sort by expert that keeps the tokens' order. A CTA's tokens are bits of one mask per expert and 32 tokens in
 // shared memory, set with OR -- no order of arrival can change it --; a token's rank inside the CTA is a population count. One CTA does
 // up to 128 tokens alone; more take three launches: selection with a count per CTA and expert, prefix sums over the CTAs, placement.
-// Bound by launches and the length of the selection's chain (64 x 64, 8 chosen: 6.5 us) and its instructions (16000 x 256: 21.5), not by the logits' bytes.
+// Bound by launches and the length of the selection's chain (64 x 64, 8 chosen: 6.3 us) and its instructions (16000 x 256: 23.6), not by the logits' bytes.
 #include <cuda_runtime.h>
 
 #include <type_traits>

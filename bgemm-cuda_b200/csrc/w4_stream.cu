@@ -80,7 +80,8 @@ __host__ __device__ constexpr int w4_pitch() { return kW4ChunkBlocks * (4 / GW) 
 
 // Warps an SM is meant to hold. Registers spill at what 24 leave each with five octets of fp16 rows (28672 x 8192 on 8 rows in
 // groups of 64: 47 us, 40 with 20 warps; bf16 31.1 and 32.3), with four scale groups a block (in groups of 32: 58 us, 49 with 16; fp16
-// 73 and 56), and with two where eight warps share K (8192 x 8192 on 4 rows 14.6 us, 12.4 with 16, on two tiles an SM anyway).
+// 73 and 56), and with two where eight warps share K (8192 x 8192 on 4 rows 14.6 us, 12.4 with 16, on two tiles an SM anyway). In groups of
+// 32 most variants still spill with 16 (up to 92 bytes stored and 120 loaded a thread).
 template <typename T>
 __host__ __device__ constexpr int w4_resident_warps(int W, int H, int GW) { return H > 2 && (GW == 1 || (GW == 2 && W == 8)) ? 16 : (H > 4 && W4Type<T>::kMagicValue == 1024.f ? 20 : 24); }
 

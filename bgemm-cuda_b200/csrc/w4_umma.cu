@@ -17,7 +17,7 @@
 // in a fixed order.
 //
 // The weight is rounded once to 16 bits, because the scale changes along K and the accumulator cannot: (q - z) s has up to
-// 15 significant bits, r16 keeps 11 (8). Sums are 32-bit.
+// 15 (bf16: 12) significant bits, r16 keeps 11 (8). Sums are 32-bit. Callers that want no weight rounded say so and get the streaming kernel.
 //
 // Tensor memory: 256 accumulator columns as two halves of 128 (a tile of up to 128 rows takes one of them, so its epilogue
 // runs under the next tile's products; a wider one takes both) + 4 operand stages of 64 columns (128 weight columns each).

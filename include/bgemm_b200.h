@@ -337,6 +337,7 @@ int64_t bgemm_w4_row_bytes(int64_t K);
  *   symmetric != 0: s = r16(max |w| * fl(1/7)), z = 8 (`zeros` is not written and may be NULL)
  *   symmetric == 0: lo = min(0, min w), hi = max(0, max w), s = r16((hi - lo) * fl(1/15)), z = clamp(rint(-lo / s), 0, 15)
  *   q = clamp(rint(w / s) + z, 0, 15), ties to even, in 32-bit arithmetic; where s is 0, q = z (8 or 0).
+ * Weights whose s is no finite number of scale_dtype (fp32 or bf16 ones above 4.5e5 with fp16 scales) have no such form: s is Inf.
  * `batch` matrices, `src_batch_stride` elements apart, fill planes, scales and zeros one behind the other.             */
 int bgemm_w4_quantize(void* stream, const void* src, int src_dtype, int64_t M, int64_t K, int64_t ld, int group, int symmetric,
                       int scale_dtype, void* plane, void* scales, uint8_t* zeros, int64_t batch, int64_t src_batch_stride);
